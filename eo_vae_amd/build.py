@@ -16,6 +16,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libeovae_hip.so')
 ARCH = 'gfx950'
+# hipcc -O3 turns scalar float code into v_pk_{add,mul,fma}_f32 by itself; some of their forms have returned wrong results
+# on this hardware now and then, so device code is built without them (the host pass warns that it does not know the feature)
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def sources():
@@ -47,6 +50,8 @@ def build(force: bool = False, verbose: bool = True) -> str:
                         for h in glob.glob(os.path.join(CSRC, '*.h')))):
             continue
         cmd = [hipcc, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-c', src, '-o', obj]
+        if src.endswith('.hip'):
+            cmd[1:1] = NO_PACKED_FP32
         if os.environ.get('EOVAE_BUILD_PARKED') == '1':    # the measured-and-parked kernels too (csrc/eovae_common.h); use --force
             cmd.insert(1, '-DEOVAE_PARKED=1')
         if verbose:
