@@ -1,0 +1,421 @@
+// Backward of the token attention (token_attn_common.h), without float atomics: two passes that each own their outputs.
+//
+//   P_m  = exp2(S_m - lse_m)            dA = dO V^T            w = (1, -lambda)
+//   dS_m = P_m o (w_m dA - delta_m)     delta_m = w_m sum_d dO o O_m
+//   dQ_m = scale dS_m K_m    dK_m = scale dS_m^T Q_m    dV = (sum_m w_m P_m)^T dO
+//   dbias[bucket] = sum of dS_0 (+ dS_1) over its pairs       dlambda = - sum dO o O_1
+//
+// attn_dq: a wave owns 32 queries and walks the keys; it also forms delta from O (for the second pass), the bias gradient's
+// partial sums (pairs of one distance lie on a diagonal of the score tile) and lambda's.  attn_dkv: a wave owns 32 keys and
+// walks the queries of every head that shares its key head, so shared heads' gradients are summed in a fixed order.  The
+// scores are formed in both passes (7 products instead of 5): the price of bit-reproducible gradients without a
+// [queries][keys] buffer.
+#include <math.h>
+#include "token_attn_common.h"
+
+using namespace tok;
+
+namespace {
+
+constexpr int SCR = TILE / 2 + 1;         // scratch row of a wave's 32 x 32 score-gradient tile (+ 1: diagonals spread over the banks)
+
+template <typename T, int D, int MAPS>
+__global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
+  using TK = Tile<T, D>;
+  constexpr int W = D / MAPS;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char *lk = lds, *lv = lds + TK::BYTES;
+  float* tab = (float*)(lds + 2 * TK::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach, ndiag = 2 * reach + 1;
+  float* diag = tab + ntab + wave * ndiag;                       // [4][2 reach + 1]: sums by distance, |distance| < reach used
+  float* scr = tab + ntab + 4 * ndiag + wave * 32 * SCR;
+  const int nbh = p.B * p.H, tiles = (p.Sq + 127) / 128;
+  const int tile = tiles - 1 - (int)blockIdx.x / nbh;
+  int b, hk, h;
+  split_bh(p, (int)blockIdx.x % nbh, b, hk, h);
+  const int row0 = tile * 128, limit = key_limit(p, b), start = start_of(p, b);
+  const int rlast = min(row0 + 128, p.Sq) - 1;
+  int kend = limit;
+  if (p.causal) kend = min(kend, start + rlast + 1);
+  const int qrow = row0 + 32 * wave + (lane & 31);
+  const bool live = qrow < p.Sq;
+  const int qlo = start + row0 + 32 * wave, qhi = qlo + 31, qpos = start + qrow;
+  const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
+  const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qrow * p.qs;
+  const size_t orow = (((size_t)b * p.Sq + qrow) * p.H + h) * D;
+  Frag<T> qf[D / 16], gf[D / 16];
+  float lam = 0.f, d1 = 0.f, d2 = 0.f;
+  if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    qf[i] = frag_global(qp, i, lane, live);
+    gf[i] = frag_global((const T*)p.d_o + orow, i, lane, live);
+    const Frag<T> of = frag_global((const T*)p.o + orow, i, lane, live);
+    if constexpr (MAPS == 2) {
+      const Frag<T> o2 = frag_global((const T*)p.o2 + orow, i, lane, live);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        d1 += (float)gf[i].x[e] * ((float)of.x[e] + lam * (float)o2.x[e]);
+        d2 += (float)gf[i].x[e] * (float)o2.x[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d1 += (float)gf[i].x[e] * (float)of.x[e];
+    }
+  }
+  d1 += other_half(d1);
+  d2 += other_half(d2);
+  float lse[MAPS], delta[MAPS];
+  delta[0] = d1;
+  if constexpr (MAPS == 2) delta[1] = -lam * d2;
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) {
+    const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + qrow;
+    lse[a] = live ? p.lse[at] : INFINITY;
+    if (live && half == 0) p.delta[at] = delta[a];
+  }
+  if (p.bk.n) {
+    fill_bias(p, tab, h, tid, 256);
+    if (p.part)
+      for (int i = lane; i < ndiag; i += 64) diag[i] = 0.f;
+  }
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
+  const float c = p.scale * LOG2E;
+  float far_l = 0.f, far_r = 0.f;
+  u32x4 rk[TK::PER], rv[TK::PER];
+  if (kend > 0) {
+    TK::fetch(rk, kb, p.ks, 0, limit, tid);
+    TK::fetch(rv, vb, p.vs, 0, limit, tid);
+  }
+  for (int k0 = 0; k0 < kend; k0 += TILE) {
+    __syncthreads();
+    TK::put(lk, rk, tid);
+    TK::put(lv, rv, tid);
+    __syncthreads();
+    if (k0 + TILE < kend) {
+      TK::fetch(rk, kb, p.ks, k0 + TILE, limit, tid);
+      TK::fetch(rv, vb, p.vs, k0 + TILE, limit, tid);
+    }
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      const int key0 = k0 + 32 * t, klast = key0 + 31;
+      if (key0 >= kend || (p.causal && key0 > qhi)) continue;
+      const bool whole = klast < limit && (!p.causal || klast <= qlo);
+      const float* tb = nullptr;
+      float far = 0.f;
+      int side = 0;
+      if (p.bk.n) {
+        if (klast - qlo <= -reach) far = tab[PAD], side = -1;
+        else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
+        else tb = tab + (reach + PAD) + key0 - qpos;
+      }
+      f32x16 da = zero16();
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lv, 32 * t, i, lane), gf[i], da);
+      f32x16 both;
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        f32x16 s = zero16();
+#pragma unroll
+        for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lk, 32 * t, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int k = acc_row(r, half);
+          float e = exp2_(s[r] * c + (tb ? tb[k] : far) - lse[a]);
+          if (!whole && (key0 + k >= limit || (p.causal && key0 + k > qpos))) e = 0.f;
+          s[r] = e * ((a == 0 ? da[r] : -lam * da[r]) - delta[a]);
+        }
+        if (a == 0) both = s;
+        else both += s;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> sf;
+          to_frag(sf, s, 8 * u);
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j)
+            acc[a * (W / 32) + j] = mma(TK::frag_t(lk, 32 * t + 16 * u, a * W + 32 * j, lane), sf, acc[a * (W / 32) + j]);
+        }
+      }
+      if (p.part) {
+        if (side) {
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += both[r];
+          if (side < 0) far_l += sum;
+          else far_r += sum;
+        } else {
+          // rows = this wave's queries, columns = keys; then lane l sums diagonal key - query = l - 31 (63 of them)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) scr[(lane & 31) * SCR + acc_row(r, half)] = both[r];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          const int off = lane - 31;
+          float sum = 0.f;
+          for (int q = 0; q < 32; ++q) {
+            const int k = q + off;
+            if (k >= 0 && k < 32) sum += scr[q * SCR + k];
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          const int rel = key0 - qlo + off;
+          if (off > 31) sum = 0.f;                                 // lane 63: no diagonal
+          if (rel <= -reach) far_l += sum;
+          else if (rel >= reach) far_r += sum;
+          else if (off <= 31) diag[rel + reach] += sum;             // one lane per distance
+        }
+      }
+    }
+  }
+  if (live) {
+    T* dq = (T*)p.dq + orow;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store4(dq + 32 * j + 8 * g + 4 * half, p.scale * acc[j][4 * g], p.scale * acc[j][4 * g + 1], p.scale * acc[j][4 * g + 2],
+               p.scale * acc[j][4 * g + 3]);
+  }
+  // partial sums of this block: bucket sums of the four waves' distances, lambda
+  const size_t slot = ((size_t)h * p.B + b) * tiles + tile;
+  if (p.part) {
+    __syncthreads();
+    float* fars = scr;
+    far_l = wave_sum(far_l);
+    far_r = wave_sum(far_r);
+    if (lane == 0) {
+      fars[0] = far_l;
+      fars[1] = far_r;
+    }
+    __syncthreads();
+    const float* d0 = tab + ntab;
+    const float* f0 = tab + ntab + 4 * ndiag;
+    for (int u = tid; u < p.bk.n; u += 256) {
+      const int right = p.bk.two_sided && u >= p.bk.side, i = right ? u - p.bk.side : u, last = p.bk.side - 1;
+      auto lo = [&](int x) { return x <= p.bk.exact ? x : p.bk.border[x - p.bk.exact - 1]; };
+      const int a = lo(i), z = i == last ? reach : lo(i + 1);         // distances a .. z - 1 (z = reach: the far sums hold the rest)
+      float sum = 0.f;
+      for (int w = 0; w < 4; ++w) {
+        for (int n = a; n < z; ++n) {
+          if (!right || n > 0) sum += d0[w * ndiag + reach + (right ? n : -n)];
+          if (!p.bk.two_sided && n == 0)
+            for (int e = 1; e < reach; ++e) sum += d0[w * ndiag + reach + e];     // one-sided: everything ahead is distance 0
+        }
+        if (i == last) sum += right ? f0[w * 32 * SCR + 1] : f0[w * 32 * SCR];
+        if (!p.bk.two_sided && i == 0) sum += f0[w * 32 * SCR + 1];
+      }
+      p.part[slot * p.bk.n + u] = sum;
+    }
+  }
+  if constexpr (MAPS == 2) {
+    if (p.lam_part) {
+      const float x = wave_sum(half == 0 && live ? d2 : 0.f);
+      __shared__ float lams[4];
+      if (lane == 0) lams[wave] = x;
+      __syncthreads();
+      if (tid == 0) p.lam_part[slot] = -(lams[0] + lams[1] + lams[2] + lams[3]);
+    }
+  }
+}
+
+template <typename T, int D, int MAPS>
+__global__ __launch_bounds__(256) void attn_dkv_kernel(const Params p) {
+  using TK = Tile<T, D>;
+  constexpr int W = D / MAPS;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char *lq = lds, *lg = lds + TK::BYTES;
+  float* rows = (float*)(lds + 2 * TK::BYTES);                    // [MAPS][2][TILE]: lse, delta
+  float* tab = rows + MAPS * 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
+  const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * 128, b = j0 / p.Hkv, hk = j0 % p.Hkv;
+  const int limit = key_limit(p, b), start = start_of(p, b);
+  const int krow = kblock + 32 * wave + (lane & 31), klo = kblock + 32 * wave, khi = klo + 31;
+  const bool live = krow < limit;
+  const T* kp = (const T*)p.k + b * p.kb + hk * p.kh + (long long)krow * p.ks;
+  const T* vp = (const T*)p.v + b * p.vb + hk * p.vh + (long long)krow * p.vs;
+  Frag<T> kf[D / 16], vf[D / 16];
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    kf[i] = frag_global(kp, i, lane, live);
+    vf[i] = frag_global(vp, i, lane, live);
+  }
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    dk[j] = zero16();
+    dv[j] = zero16();
+  }
+  const float c = p.scale * LOG2E;
+  int first = 0;                                                  // first query row that sees a key of this block
+  if (p.causal) first = max(0, kblock - start) / TILE * TILE;
+  const int per = kblock < limit && first < p.Sq ? (p.Sq - first + TILE - 1) / TILE : 0, total = per * G;
+  u32x4 rq[TK::PER], rg[TK::PER];
+  float rl[MAPS], rd[MAPS];
+  const auto fetch = [&](int it) {
+    const int h = hk * G + it / per, q0 = first + it % per * TILE;
+    TK::fetch(rq, (const T*)p.q + b * p.qb + h * p.qh, p.qs, q0, p.Sq, tid);
+    TK::fetch(rg, (const T*)p.d_o + ((size_t)b * p.Sq * p.H + h) * D, (long long)p.H * D, q0, p.Sq, tid);
+    if (tid < TILE)
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + q0 + tid;
+        rl[a] = q0 + tid < p.Sq ? p.lse[at] : INFINITY;
+        rd[a] = q0 + tid < p.Sq ? p.delta[at] : 0.f;
+      }
+  };
+  if (total > 0) fetch(0);
+  float lam = 0.f;
+  for (int it = 0; it < total; ++it) {
+    const int h = hk * G + it / per, q0 = first + it % per * TILE;
+    __syncthreads();
+    TK::put(lq, rq, tid);
+    TK::put(lg, rg, tid);
+    if (tid < TILE)
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        rows[a * 2 * TILE + tid] = rl[a];
+        rows[a * 2 * TILE + TILE + tid] = rd[a];
+      }
+    if (it % per == 0) {
+      if (p.bk.n) fill_bias(p, tab, h, tid, 256);
+      if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+    }
+    __syncthreads();
+    if (it + 1 < total) fetch(it + 1);
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      const int r0 = q0 + 32 * t, qlo = start + r0, qhi = qlo + 31;
+      if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
+      const bool whole = khi < limit && (!p.causal || khi <= qlo);
+      const float* tb = nullptr;
+      float far = 0.f;
+      if (p.bk.n) {
+        if (khi - qlo <= -reach) far = tab[PAD];
+        else if (klo - qhi >= reach) far = tab[2 * (reach + PAD)];
+        else tb = tab + (reach + PAD) + krow - qlo;
+      }
+      f32x16 da = zero16(), mix;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lg, 32 * t, i, lane), vf[i], da);
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        f32x16 s = zero16();
+#pragma unroll
+        for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lq, 32 * t, a * (W / 16) + i, lane), kf[a * (W / 16) + i], s);
+        const float* ls = rows + a * 2 * TILE + 32 * t;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int q = acc_row(r, half);
+          float e = exp2_(s[r] * c + (tb ? tb[-q] : far) - ls[q]);
+          if (!whole && (krow >= limit || (p.causal && krow > qlo + q))) e = 0.f;
+          if (a == 0) mix[r] = e;
+          else mix[r] -= lam * e;
+          s[r] = e * ((a == 0 ? da[r] : -lam * da[r]) - ls[TILE + q]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> sf;
+          to_frag(sf, s, 8 * u);
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j)
+            dk[a * (W / 32) + j] = mma(TK::frag_t(lq, 32 * t + 16 * u, a * W + 32 * j, lane), sf, dk[a * (W / 32) + j]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Frag<T> pf;
+        to_frag(pf, mix, 8 * u);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) dv[j] = mma(TK::frag_t(lg, 32 * t + 16 * u, 32 * j, lane), pf, dv[j]);
+      }
+    }
+  }
+  if (krow < p.Sk) {
+    const size_t at = (((size_t)b * p.Sk + krow) * p.Hkv + hk) * D;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * j + 8 * g + 4 * half;
+        store4((T*)p.dk + at + d, p.scale * dk[j][4 * g], p.scale * dk[j][4 * g + 1], p.scale * dk[j][4 * g + 2], p.scale * dk[j][4 * g + 3]);
+        store4((T*)p.dv + at + d, dv[j][4 * g], dv[j][4 * g + 1], dv[j][4 * g + 2], dv[j][4 * g + 3]);
+      }
+  }
+}
+
+// table gradient [n][H] and lambda gradient [H] from the blocks' partial sums; one wave per value, fp64, fixed order
+__global__ __launch_bounds__(64) void attn_fold_kernel(const float* part, const float* lam_part, void* dbias, void* dlam, int n, int H,
+                                                       int slots, int bias_f32, int lam_f32) {
+  const int h = (int)blockIdx.x % H, u = (int)blockIdx.x / H, lane = threadIdx.x;
+  const bool lam = u == n;
+  double sum = 0.0;
+  for (int s = lane; s < slots; s += 64) {
+    const size_t at = (size_t)h * slots + s;
+    sum += lam ? lam_part[at] : part[at * n + u];
+  }
+  sum = wave_sum_d(sum);
+  if (lane) return;
+  void* out = lam ? dlam : dbias;
+  const size_t at = lam ? (size_t)h : (size_t)u * H + h;
+  if (lam ? lam_f32 : bias_f32) ((float*)out)[at] = (float)sum;
+  else ((__bf16*)out)[at] = (__bf16)(float)sum;
+}
+
+struct Sizes {
+  size_t delta, part, lam;      // floats
+  int slots;
+};
+Sizes sizes_of(const Params& p, int maps, bool dbias, bool dlam) {
+  Sizes s;
+  s.slots = p.B * ((p.Sq + 127) / 128);
+  s.delta = ((size_t)p.B * p.H * maps * p.Sq + 3) & ~(size_t)3;
+  s.part = dbias ? ((size_t)s.slots * p.H * p.bk.n + 3) & ~(size_t)3 : 0;
+  s.lam = dlam ? (size_t)s.slots * p.H : 0;
+  return s;
+}
+
+template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_attention* d, hipStream_t st) {
+  const char* who = "token_attention_bwd";
+  const Sizes s = sizes_of(p, MAPS, d->dbias, d->dlam);
+  const size_t need = 4 * (s.delta + s.part + s.lam);
+  EOVAE_CHECK_ARG(d->ws && d->ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", who, d->ws_bytes, need);
+  p.delta = (float*)d->ws;
+  if (d->dbias) p.part = p.delta + s.delta;
+  if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
+  const size_t tiles = 2 * (size_t)Tile<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
+  const size_t sums = d->dbias ? 4 * (4 * (size_t)(2 * p.bk.reach + 1) + 4 * 32 * SCR) : 0;
+  int rc = launch(attn_dq_kernel<T, D, MAPS>, (size_t)((p.Sq + 127) / 128) * p.B * p.H, 256, tiles + tab + sums, p, st, who);
+  if (rc) return rc;
+  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 4 * MAPS * 2 * TILE, p, st, who);
+  if (rc) return rc;
+  const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);
+  if (outs == 0) return EOVAE_OK;
+  hipLaunchKernelGGL(attn_fold_kernel, dim3((unsigned)(p.H * outs)), dim3(64), 0, st, p.part, p.lam_part, d->dbias, d->dlam, nb, p.H, s.slots,
+                     p.bias_f32, p.lam_f32);
+  EOVAE_CHECK_LAUNCH(who);
+  return EOVAE_OK;
+}
+
+}  // namespace
+
+size_t tok_fwd_workspace(const eovae_token_attention* d, const Params& p);
+
+extern "C" {
+size_t eovae_token_attention_workspace(const eovae_token_attention* d, int backward) {
+  Params p;
+  if (make_params(d, p, "token_attention_workspace", 0)) return 0;
+  if (!backward) return tok_fwd_workspace(d, p);
+  const Sizes s = sizes_of(p, d->maps, d->bias != nullptr, d->maps == 2);
+  return 4 * (s.delta + s.part + s.lam);
+}
+int eovae_token_attention_bwd(const eovae_token_attention* d, void* stream) {
+  Params p;
+  const int rc = make_params(d, p, "token_attention_bwd", 1);
+  if (rc) return rc;
+  return TOK_DISPATCH(d, run_bwd, p, d, (hipStream_t)stream);
+}
+}

@@ -1,0 +1,308 @@
+// Shared device code of the token attention kernels (token_attn_fwd.hip, token_attn_bwd.hip).
+//
+//   S_m = scale * Q_m K_m^T + bias[bucket(key position - query position)][head]      m = 0 (and 1: differential attention)
+//   O   = softmax(S_0) V                or        (softmax(S_0) - lambda[head] softmax(S_1)) V
+//
+// One fragment shape serves every product: v_mfma_f32_32x32x16 on bf16, and for fp32 eight v_mfma_f32_32x32x2 on the SAME
+// lane layout (lane l holds row l % 32 and the eight k of its half l / 32; the order of k inside an instruction is free as
+// long as both operands agree on it).  The accumulator leaves lane l with column l % 32 and the rows 8 (r / 4) + 4 (l / 32)
+// + r % 4, r < 16: eight consecutive registers are a B operand of the next product whose k run {4h..4h+3, 8+4h..8+4h+3}
+// (h = l / 32), so probabilities and score gradients go from one product into the next without leaving their lane, as long
+// as the A operand is read in that order (frag_t below).
+#pragma once
+#include <math.h>
+#include "eovae_common.h"
+#include "../../include/eovae_hip.h"
+
+namespace tok {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int MAX_BUCKETS = 128;       // per side: at most 64 borders behind the exact half
+constexpr int MAX_REACH = 1024;
+constexpr int TILE = 64;               // rows of a staged tile
+constexpr int PAD = 32 + TILE;         // a 32 x TILE tile that touches |rel| < reach stays inside [-reach - PAD, reach + PAD]
+
+// Buckets of one side: n < exact -> n, else exact + #{borders <= n}.  reach: first distance of the last bucket (everything
+// at and behind it shares one value).  two_sided: positive distances use the second half of the table.
+struct Buckets {
+  int n, side, exact, nborders, reach, two_sided;
+  int border[MAX_BUCKETS / 2];
+};
+
+__device__ __forceinline__ int bucket_of(const Buckets& t, int rel) {
+  int n = t.two_sided ? (rel < 0 ? -rel : rel) : (rel < 0 ? -rel : 0);
+  int b = n;
+  if (n >= t.exact) {
+    b = t.exact;
+    for (int i = 0; i < t.nborders; ++i) b += n >= t.border[i] ? 1 : 0;
+  }
+  return b + (t.two_sided && rel > 0 ? t.side : 0);
+}
+
+struct Params {
+  const void *q, *k, *v, *o2, *d_o, *o;
+  void *out, *out2;
+  void *dq, *dk, *dv;
+  const void *bias, *lam;
+  const int *kv_len, *q_start;
+  float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain (+inf: nothing visible); delta likewise
+  long long qb, qs, qh, kb, ks, kh, vb, vs, vh;   // element strides: batch, token, head
+  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, chunk;
+  float scale;
+  Buckets bk;
+};
+
+template <typename T> struct Frag;
+template <> struct Frag<__bf16> { bf16x8 x; };
+template <> struct Frag<float> { f32x8 x; };
+
+__device__ __forceinline__ f32x16 mma(const Frag<__bf16>& a, const Frag<__bf16>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.x, b.x, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[i], b.x[i], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ float ldf(const void* p, size_t i, int is_f32) {
+  return is_f32 ? ((const float*)p)[i] : (float)((const __bf16*)p)[i];
+}
+
+// ---- staged tiles: TILE rows of D elements, 16-byte chunks, chunk index XORed with swz(row) ----
+// Eight consecutive rows at one chunk index (a fragment read: lanes = rows) fall into eight different 16-byte bank groups,
+// and four consecutive rows times two consecutive chunks (a transposed 16-bit read) cover all 128 bytes once.
+template <typename T, int D> struct Tile {
+  static constexpr int ROWB = D * (int)sizeof(T);
+  static constexpr int CH = ROWB / 16;                       // chunks per row: 4 .. 32
+  static constexpr int BYTES = TILE * ROWB;
+  static constexpr int PER = TILE * CH / 256;                // chunks per thread of a 256-thread block (1 .. 8)
+  static __device__ __forceinline__ int swz(int row) {
+    return CH >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : ((row & 2) | ((row >> 2) & 1));
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
+
+  // rows row0 .. row0 + TILE - 1 of a strided matrix; rows >= limit read as zero (never touched in memory)
+  static __device__ __forceinline__ void fetch(u32x4 (&r)[PER], const T* base, long long stride, int row0, int limit, int tid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + 256 * i, row = c / CH, ch = c % CH;
+      u32x4 z = {0, 0, 0, 0};
+      if (row0 + row < limit) z = *(const u32x4*)((const char*)(base + (long long)(row0 + row) * stride) + ch * 16);
+      r[i] = z;
+    }
+  }
+  static __device__ __forceinline__ void put(char* lds, const u32x4 (&r)[PER], int tid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = tid + 256 * i;
+      *(u32x4*)(lds + at(c / CH, c % CH)) = r[i];
+    }
+  }
+  // operand fragment: lane holds row (row0 + l % 32), columns 16 s + 8 (l / 32) .. + 7
+  static __device__ __forceinline__ Frag<T> frag(const char* lds, int row0, int s, int lane) {
+    const int row = row0 + (lane & 31), half = lane >> 5;
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      f.x = *(const bf16x8*)(lds + at(row, 2 * s + half));
+    } else {
+      const f32x4 a = *(const f32x4*)(lds + at(row, 4 * s + 2 * half)), b = *(const f32x4*)(lds + at(row, 4 * s + 2 * half + 1));
+      f.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+  }
+  // transposed operand: lane holds COLUMN col0 + l % 32 and the rows row0 + {4h .. 4h + 3, 8 + 4h .. 8 + 4h + 3}
+  static __device__ __forceinline__ Frag<T> frag_t(char* lds, int row0, int col0, int lane) {
+    Frag<T> f;
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      // ds_read_b64_tr_b16: each 16-lane group hands in four rows of 16 columns (lane: row l / 4, columns 4 (l % 4)) and
+      // gets back, per lane, its column's four rows
+      const int g = (lane >> 4) & 1, row = row0 + 4 * half + ((lane & 15) >> 2), col = col0 + 16 * g + 4 * (lane & 3);
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const int off = (col & 7) * 2;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lds + at(row, col >> 3) + off));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lds + at(row + 8, col >> 3) + off));
+      f.x = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int col = col0 + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = row0 + 4 * half + (i & 3) + 8 * (i >> 2);
+        f.x[i] = *(const float*)(lds + at(row, col >> 2) + (col & 3) * 4);
+      }
+    }
+    return f;
+  }
+};
+
+// fragment of a row straight from global memory (row < limit, else zero)
+template <typename T> __device__ __forceinline__ Frag<T> frag_global(const T* row, int s, int lane, bool ok) {
+  Frag<T> f;
+  const int c = 16 * s + 8 * (lane >> 5);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f.x[i] = (T)0.f;
+  if (ok) {
+    if constexpr (sizeof(T) == 2) {
+      f.x = *(const bf16x8*)(row + c);
+    } else {
+      const f32x4 a = *(const f32x4*)(row + c), b = *(const f32x4*)(row + c + 4);
+      f.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  return f;
+}
+
+// eight consecutive accumulator registers as the B operand of the next product
+__device__ __forceinline__ void to_frag(Frag<__bf16>& f, const f32x16& a, int r0) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f.x[i] = (__bf16)a[r0 + i];
+}
+__device__ __forceinline__ void to_frag(Frag<float>& f, const f32x16& a, int r0) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f.x[i] = a[r0 + i];
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<__bf16>(__bf16* p, float a, float b, float c, float d) {
+  bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+  *(bf16x4*)p = v;
+}
+template <> __device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+  f32x4 v = {a, b, c, d};
+  *(f32x4*)p = v;
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+// the value of the other half's lane with the same column
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ int key_limit(const Params& p, int b) {
+  if (!p.kv_len) return p.Sk;
+  const int n = p.kv_len[b];
+  return n < 0 ? 0 : (n > p.Sk ? p.Sk : n);
+}
+// position of query row 0 among the keys; clamped so that differences of positions stay inside 32 bits
+__device__ __forceinline__ int start_of(const Params& p, int b) {
+  const int s = p.q_start ? p.q_start[b] : p.start;
+  return s < -(1 << 30) ? -(1 << 30) : (s > (1 << 30) ? (1 << 30) : s);
+}
+
+// head's bias by distance, log2 domain: tab[rel + reach + PAD], rel in [-reach - PAD, reach + PAD]
+__device__ __forceinline__ void fill_bias(const Params& p, float* tab, int head, int tid, int nthreads) {
+  const int span = p.bk.reach + PAD;
+  for (int i = tid; i <= 2 * span; i += nthreads)
+    tab[i] = ldf(p.bias, (size_t)bucket_of(p.bk, i - span) * p.H + head, p.bias_f32) * LOG2E;
+}
+static inline int bias_entries(const Buckets& b) { return b.n ? 2 * (b.reach + PAD) + 1 : 0; }
+
+// heads that share key heads sit next to each other in launch order with stride B * Hkv: with B * Hkv a multiple of 8 the
+// blocks that read one key head land on one XCD and its L2 (workgroups go round the XCDs in launch order)
+__device__ __forceinline__ void split_bh(const Params& p, int j, int& b, int& hk, int& h) {
+  const int n = p.B * p.Hkv, g = j / n, r = j % n;
+  b = r / p.Hkv;
+  hk = r % p.Hkv;
+  h = hk * (p.H / p.Hkv) + g;
+}
+
+// ---- host side ----
+// checks a descriptor and turns it into kernel parameters; null pointers are allowed only where the header says so
+static inline int make_params(const eovae_token_attention* d, Params& p, const char* who, int backward) {
+  EOVAE_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
+  EOVAE_CHECK_ARG(d->dtype == EOVAE_F32 || d->dtype == EOVAE_BF16, "%s: dtype %d (0 fp32, 1 bf16)", who, d->dtype);
+  EOVAE_CHECK_ARG(d->maps == 1 || d->maps == 2, "%s: %d softmax maps (1 or 2)", who, d->maps);
+  EOVAE_CHECK_ARG(d->dim == 64 || d->dim == 128 || (d->dim == 32 && d->maps == 1), "%s: head width %d with %d map(s) (32, 64 or 128; two maps: 64 or 128)",
+                  who, d->dim, d->maps);
+  EOVAE_CHECK_ARG(d->batch >= 1 && d->sq >= 1 && d->sk >= 1 && d->heads >= 1 && d->kv_heads >= 1 && d->sq <= (1 << 28) && d->sk <= (1 << 28) &&
+                      d->batch <= (1 << 20) && d->heads <= (1 << 16),
+                  "%s: batch %d, queries %d, keys %d, heads %d / %d out of range", who, d->batch, d->sq, d->sk, d->heads, d->kv_heads);
+  EOVAE_CHECK_ARG(d->heads % d->kv_heads == 0, "%s: %d heads over %d key heads", who, d->heads, d->kv_heads);
+  const long long es = d->dtype == EOVAE_F32 ? 4 : 2;
+  const long long* st[3] = {d->q_strides, d->k_strides, d->v_strides};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j)
+      EOVAE_CHECK_ARG(st[i][j] >= 0 && st[i][j] * es % 16 == 0, "%s: stride %lld is negative or no multiple of 16 bytes", who, st[i][j]);
+  const void* ptrs[] = {d->q, d->k, d->v, d->out, d->out2, d->d_out, d->dq, d->dk, d->dv, d->ws};
+  for (const void* x : ptrs) EOVAE_CHECK_ARG((size_t)x % 16 == 0, "%s: a tensor is not 16-byte aligned", who);
+  EOVAE_CHECK_ARG(d->q && d->k && d->v && d->out, "%s: null q, k, v or out", who);
+  EOVAE_CHECK_ARG(d->maps == 1 || d->lam, "%s: two maps need lambda", who);
+  EOVAE_CHECK_ARG(isfinite(d->scale), "%s: scale is not finite", who);
+  if (backward) {
+    EOVAE_CHECK_ARG(d->lse && d->d_out && d->dq && d->dk && d->dv, "%s: null lse, d_out, dq, dk or dv", who);
+    EOVAE_CHECK_ARG(d->maps == 1 || d->out2, "%s: two maps need out2 of the forward", who);
+    EOVAE_CHECK_ARG(!d->dbias || d->bias, "%s: dbias without a bias table", who);
+    EOVAE_CHECK_ARG(!d->dlam || d->maps == 2, "%s: dlam with one map", who);
+  }
+  p.q = d->q; p.k = d->k; p.v = d->v; p.o2 = d->out2; p.o = d->out; p.d_o = d->d_out;
+  p.out = d->out; p.out2 = d->out2;
+  p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;
+  p.bias = d->bias; p.lam = d->lam;
+  p.kv_len = d->kv_len; p.q_start = d->query_start;
+  p.lse = d->lse; p.delta = nullptr; p.part = nullptr; p.lam_part = nullptr;
+  p.qb = d->q_strides[0]; p.qs = d->q_strides[1]; p.qh = d->q_strides[2];
+  p.kb = d->k_strides[0]; p.ks = d->k_strides[1]; p.kh = d->k_strides[2];
+  p.vb = d->v_strides[0]; p.vs = d->v_strides[1]; p.vh = d->v_strides[2];
+  p.B = d->batch; p.Sq = d->sq; p.Sk = d->sk; p.H = d->heads; p.Hkv = d->kv_heads; p.start = d->start; p.causal = d->causal ? 1 : 0;
+  p.bias_f32 = d->bias_dtype == EOVAE_F32; p.lam_f32 = d->lam_dtype == EOVAE_F32;
+  p.splits = 1; p.chunk = 0;
+  p.scale = d->scale;
+  Buckets& t = p.bk;
+  t.n = t.side = t.exact = t.nborders = t.reach = t.two_sided = 0;
+  if (d->bias) {
+    EOVAE_CHECK_ARG(d->buckets >= 2 && d->buckets <= MAX_BUCKETS, "%s: %d buckets (2 .. %d)", who, d->buckets, MAX_BUCKETS);
+    t.n = d->buckets;
+    t.two_sided = d->two_sided ? 1 : 0;
+    t.side = t.two_sided ? t.n / 2 : t.n;
+    EOVAE_CHECK_ARG(t.side >= 2 && (!t.two_sided || t.n % 2 == 0), "%s: %d buckets over %d side(s)", who, t.n, t.two_sided + 1);
+    t.exact = t.side / 2;
+    t.nborders = t.side - t.exact - 1;
+    EOVAE_CHECK_ARG(t.nborders == 0 || d->borders, "%s: null borders", who);
+    t.reach = t.exact;
+    for (int i = 0; i < t.nborders; ++i) {
+      EOVAE_CHECK_ARG(d->borders[i] >= t.reach && d->borders[i] <= MAX_REACH, "%s: border %d of %d falls, or lies beyond %d", who, i, t.nborders, MAX_REACH);
+      t.border[i] = t.reach = d->borders[i];
+    }
+  }
+  return EOVAE_OK;
+}
+
+// more than 64 KiB of LDS per block has to be asked for
+template <typename K> static inline int launch(K kernel, size_t blocks, int threads, size_t lds, const Params& p, hipStream_t st, const char* who) {
+  EOVAE_CHECK_ARG(blocks <= 0x7fffffff, "%s: %zu blocks", who, blocks);
+  EOVAE_CHECK_ARG(lds <= 160 * 1024, "%s: %zu bytes of LDS", who, lds);
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) {
+      eovae_set_error("%s: %zu bytes of LDS refused: %s", who, lds, hipGetErrorString(e));
+      return EOVAE_ERR_LAUNCH;
+    }
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, p);
+  EOVAE_CHECK_LAUNCH(who);
+  return EOVAE_OK;
+}
+
+}  // namespace tok
+
+// calls F<T, D, MAPS>(args...) for the descriptor's type, width and maps (make_params has checked the combination)
+#define TOK_DISPATCH(d, F, ...)                                                                                          \
+  ((d)->dtype == EOVAE_F32                                                                                              \
+       ? ((d)->maps == 2 ? ((d)->dim == 64 ? F<float, 64, 2>(__VA_ARGS__) : F<float, 128, 2>(__VA_ARGS__))               \
+                         : ((d)->dim == 32 ? F<float, 32, 1>(__VA_ARGS__)                                                \
+                                           : (d)->dim == 64 ? F<float, 64, 1>(__VA_ARGS__) : F<float, 128, 1>(__VA_ARGS__))) \
+       : ((d)->maps == 2 ? ((d)->dim == 64 ? F<__bf16, 64, 2>(__VA_ARGS__) : F<__bf16, 128, 2>(__VA_ARGS__))             \
+                         : ((d)->dim == 32 ? F<__bf16, 32, 1>(__VA_ARGS__)                                               \
+                                           : (d)->dim == 64 ? F<__bf16, 64, 1>(__VA_ARGS__) : F<__bf16, 128, 1>(__VA_ARGS__))))

@@ -1,0 +1,426 @@
+// Fused attention forward with bucketed relative position bias, one or two softmax maps (token_attn_common.h).
+//
+// Row form: a block owns 128 (two maps: 64) query rows of one head and walks the keys once, 64 at a time, with the running
+// maximum and sum of every row's softmax; a lane owns ONE query (its column of S^T = K Q^T), so the statistics are plain
+// registers and the other half of a column is one cross-lane exchange away.  Two maps: waves 0, 1 hold map 0, waves 2, 3
+// map 1 of the same rows (same K / V tiles, half of K's columns each) and meet once at the end.
+// Step form (few rows per key head, e.g. single tokens against a cache): the rows are the query heads that share one key
+// head times the query tokens (<= 32 per block), the four waves take different keys, the key axis is also split over blocks,
+// and a second kernel joins the partial sums.
+#include <math.h>
+#include "token_attn_common.h"
+
+using namespace tok;
+
+namespace {
+
+// One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
+// key0: position of the tile's first key; qpos: this lane's query position; limit: keys visible at all.
+template <typename T, int D, int W, int NT>
+__device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
+                                          float& m, float& l, int map, int key0, int lkey0, int limit, int qpos, int qlo, int qhi,
+                                          const float* tab, int lane) {
+  using TK = Tile<T, D>;
+  const int half = lane >> 5;
+  const float c = p.scale * LOG2E;
+  f32x16 s[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    s[t] = zero16();
+#pragma unroll
+    for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, lkey0 + 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
+  }
+  const int klast = key0 + 32 * NT - 1;
+  const bool whole = klast < limit && (!p.causal || klast <= qlo);
+  float top = -INFINITY;
+  const float* tb = nullptr;
+  float far = 0.f;
+  if (p.bk.n) {
+    const int reach = p.bk.reach;
+    if (klast - qlo <= -reach) far = tab[PAD];                              // every pair at or behind the last border
+    else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)];
+    else tb = tab + (reach + PAD) + key0 - qpos;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int k = 32 * t + acc_row(r, half);
+      float x = s[t][r] * c + (tb ? tb[k] : far);
+      if (!whole && (key0 + k >= limit || (p.causal && key0 + k > qpos))) x = -INFINITY;
+      s[t][r] = x;
+      top = fmaxf(top, x);
+    }
+  top = fmaxf(top, other_half(top));
+  const float mn = fmaxf(m, top);
+  const float base = mn == -INFINITY ? 0.f : mn;
+  const float a = exp2_(m - base);                                        // m = -inf: 0
+  m = mn;
+  float sum = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float e = exp2_(s[t][r] - base);
+      s[t][r] = e;
+      sum += e;
+    }
+  l = l * a + sum;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) acc[j] *= a;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      Frag<T> pf;
+      to_frag(pf, s[t], 8 * u);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) acc[j] = mma(TK::frag_t(lv, lkey0 + 32 * t + 16 * u, 32 * j, lane), pf, acc[j]);
+    }
+}
+
+template <typename T, int D, int MAPS>
+__global__ __launch_bounds__(256) void attn_rows_kernel(const Params p) {
+  using TK = Tile<T, D>;
+  constexpr int W = D / MAPS;                 // width of one map's queries and keys
+  constexpr int RB = 128 / MAPS;              // query rows of a block
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char *lk = lds, *lv = lds + TK::BYTES;
+  float* tab = (float*)(lds + 2 * TK::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int map = MAPS == 2 ? wave >> 1 : 0, wrow = 32 * (MAPS == 2 ? (wave & 1) : wave);
+  const int nbh = p.B * p.H, tiles = (p.Sq + RB - 1) / RB;
+  const int tile = tiles - 1 - (int)blockIdx.x / nbh;      // causal: the longest rows first
+  int b, hk, h;
+  split_bh(p, (int)blockIdx.x % nbh, b, hk, h);
+  const int row0 = tile * RB, limit = key_limit(p, b), start = start_of(p, b);
+  const int rlast = min(row0 + RB, p.Sq) - 1;
+  int kend = limit;
+  if (p.causal) kend = min(kend, start + rlast + 1);
+  const int qrow = row0 + wrow + (lane & 31);
+  const bool live = qrow < p.Sq;
+  const int qlo = start + row0 + wrow, qhi = qlo + 31, qpos = start + qrow;
+  const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
+  const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qrow * p.qs + map * W;
+  Frag<T> qf[W / 16];
+#pragma unroll
+  for (int i = 0; i < W / 16; ++i) qf[i] = frag_global(qp, i, lane, live);
+  if (p.bk.n) fill_bias(p, tab, h, tid, 256);
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
+  float m = -INFINITY, l = 0.f;
+  u32x4 rk[TK::PER], rv[TK::PER];
+  if (kend > 0) {
+    TK::fetch(rk, kb, p.ks, 0, limit, tid);
+    TK::fetch(rv, vb, p.vs, 0, limit, tid);
+  }
+  for (int k0 = 0; k0 < kend; k0 += TILE) {
+    __syncthreads();
+    TK::put(lk, rk, tid);
+    TK::put(lv, rv, tid);
+    __syncthreads();
+    if (k0 + TILE < kend) {
+      TK::fetch(rk, kb, p.ks, k0 + TILE, limit, tid);
+      TK::fetch(rv, vb, p.vs, k0 + TILE, limit, tid);
+    }
+    if (!p.causal || k0 <= qhi)
+      tile_step<T, D, W, 2>(p, lk, lv, qf, acc, m, l, map, k0, 0, limit, qpos, qlo, qhi, tab, lane);
+  }
+  l += other_half(l);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) acc[j] *= inv;
+  if (p.lse && live && half == 0)
+    p.lse[(((size_t)b * p.H + h) * MAPS + map) * p.Sq + qrow] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+  const size_t orow = (((size_t)b * p.Sq + qrow) * p.H + h) * D;
+  if constexpr (MAPS == 2) {
+    // the second map's rows meet the first's through LDS: [64 rows][D] fp32, one column of 4 floats per lane and register quad
+    float* meet = (float*)lds;
+    constexpr int MROW = D + 4;
+    __syncthreads();
+    if (map == 1) {
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * j + 8 * g + 4 * half;
+          f32x4 v = {acc[j][4 * g], acc[j][4 * g + 1], acc[j][4 * g + 2], acc[j][4 * g + 3]};
+          *(f32x4*)(meet + (wrow + (lane & 31)) * MROW + d) = v;
+          if (p.out2 && live) store4((T*)p.out2 + orow + d, v[0], v[1], v[2], v[3]);
+        }
+    }
+    __syncthreads();
+    if (map == 0 && live) {
+      const float lam = ldf(p.lam, h, p.lam_f32);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * j + 8 * g + 4 * half;
+          const f32x4 v = *(const f32x4*)(meet + (wrow + (lane & 31)) * MROW + d);
+          store4((T*)p.out + orow + d, acc[j][4 * g] - lam * v[0], acc[j][4 * g + 1] - lam * v[1], acc[j][4 * g + 2] - lam * v[2],
+                 acc[j][4 * g + 3] - lam * v[3]);
+        }
+    }
+  } else if (live) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store4((T*)p.out + orow + 32 * j + 8 * g + 4 * half, acc[j][4 * g], acc[j][4 * g + 1], acc[j][4 * g + 2], acc[j][4 * g + 3]);
+  }
+}
+
+// ---- step form ----
+// part (fp32): per (b, key head, row block, split, map): [32 rows][D] unnormalised sums, then per row (maximum, sum)
+template <int D, int MAPS> constexpr int part_floats() { return MAPS * 32 * (D + 2); }
+
+template <typename T, int D, int MAPS>
+__global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
+  using TK = Tile<T, D>;
+  constexpr int W = D / MAPS;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char *lk = lds, *lv = lds + 2 * TK::BYTES;                  // 128 keys: two tiles of K, two of V
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
+  int j = (int)blockIdx.x;
+  const int split = j % p.splits;
+  j /= p.splits;
+  const int rb = j % rblocks;
+  j /= rblocks;
+  const int hk = j % p.Hkv, b = j / p.Hkv;
+  const int row = rb * 32 + (lane & 31);
+  const bool live = row < rows;
+  const int g = live ? row / p.Sq : 0, qi = live ? row % p.Sq : 0, h = hk * G + g;
+  const int limit = key_limit(p, b), start = start_of(p, b), qpos = start + qi;
+  int kend = limit;
+  if (p.causal) kend = min(kend, start + p.Sq);
+  const int k_lo = split * p.chunk, k_hi = min(kend, k_lo + p.chunk);
+  const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
+  const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qi * p.qs;
+  // bias: bucket per distance (one byte) and the key head's rows of the table; two LDS reads per score near the query
+  unsigned char* ids = (unsigned char*)(lds + 4 * TK::BYTES);
+  const int reach = p.bk.reach;
+  float* tab = (float*)(ids + (p.bk.n ? ((2 * reach + 1 + 15) & ~15) : 0));
+  if (p.bk.n) {
+    for (int i = tid; i <= 2 * reach; i += 256) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
+    for (int i = tid; i < p.bk.n * G; i += 256) tab[i] = ldf(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32) * LOG2E;
+  }
+  Frag<T> qf[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) qf[i] = frag_global(qp, i, lane, live);
+  f32x16 acc[MAPS][D / 32];
+  float m[MAPS], l[MAPS];
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[a][i] = zero16();
+  }
+  const float c = p.scale * LOG2E;
+  u32x4 rk[2][TK::PER], rv[2][TK::PER];
+  if (k_lo < k_hi)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      TK::fetch(rk[t], kb, p.ks, k_lo + TILE * t, k_hi, tid);
+      TK::fetch(rv[t], vb, p.vs, k_lo + TILE * t, k_hi, tid);
+    }
+  for (int k0 = k_lo; k0 < k_hi; k0 += 2 * TILE) {
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      TK::put(lk + t * TK::BYTES, rk[t], tid);
+      TK::put(lv + t * TK::BYTES, rv[t], tid);
+    }
+    __syncthreads();
+    if (k0 + 2 * TILE < k_hi)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        TK::fetch(rk[t], kb, p.ks, k0 + 2 * TILE + TILE * t, k_hi, tid);
+        TK::fetch(rv[t], vb, p.vs, k0 + 2 * TILE + TILE * t, k_hi, tid);
+      }
+    const int kw = k0 + 32 * wave;                                // this wave's 32 keys
+    if (kw >= k_hi) continue;
+    char *wk = lk + (wave >> 1) * TK::BYTES, *wv = lv + (wave >> 1) * TK::BYTES;
+    const int r0 = 32 * (wave & 1);
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      f32x16 s = zero16();
+#pragma unroll
+      for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(wk, r0, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
+      float top = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int k = kw + acc_row(r, half);
+        float x = s[r] * c;
+        if (p.bk.n) {
+          int rel = k - qpos;
+          rel = rel < -reach ? -reach : (rel > reach ? reach : rel);
+          x += tab[ids[rel + reach] * G + g];
+        }
+        if (k >= k_hi || (p.causal && k > qpos)) x = -INFINITY;
+        s[r] = x;
+        top = fmaxf(top, x);
+      }
+      top = fmaxf(top, other_half(top));
+      const float mn = fmaxf(m[a], top), base = mn == -INFINITY ? 0.f : mn, al = exp2_(m[a] - base);
+      m[a] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = exp2_(s[r] - base);
+        sum += s[r];
+      }
+      l[a] = l[a] * al + sum;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[a][i] *= al;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Frag<T> pf;
+        to_frag(pf, s, 8 * u);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[a][i] = mma(TK::frag_t(wv, r0 + 16 * u, 32 * i, lane), pf, acc[a][i]);
+      }
+    }
+  }
+  // join the four waves: [wave][32 rows][D + 4] sums and [wave][32][2] statistics, one map at a time
+  constexpr int MROW = D + 4;
+  float* meet = (float*)lds;
+  float* stat = meet + 4 * 32 * MROW;
+  float* out = p.part + (size_t)blockIdx.x * part_floats<D, MAPS>();
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) {
+    __syncthreads();
+    const float lt = l[a] + other_half(l[a]);
+    const int col = lane & 31;
+    if (half == 0) {
+      stat[(wave * 32 + col) * 2] = m[a];
+      stat[(wave * 32 + col) * 2 + 1] = lt;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 v = {acc[a][i][4 * q], acc[a][i][4 * q + 1], acc[a][i][4 * q + 2], acc[a][i][4 * q + 3]};
+        *(f32x4*)(meet + (wave * 32 + col) * MROW + 32 * i + 8 * q + 4 * half) = v;
+      }
+    __syncthreads();
+    for (int i = tid; i < 32 * D / 4; i += 256) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      if (rb * 32 + r >= rows) continue;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, stat[(w * 32 + r) * 2]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      float ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = exp2_(stat[(w * 32 + r) * 2] - base);
+        ls += f * stat[(w * 32 + r) * 2 + 1];
+        sum += f * *(const f32x4*)(meet + (w * 32 + r) * MROW + d);
+      }
+      *(f32x4*)(out + (a * 32 + r) * D + d) = sum;
+      if (d == 0) {
+        out[MAPS * 32 * D + (a * 32 + r) * 2] = mm;
+        out[MAPS * 32 * D + (a * 32 + r) * 2 + 1] = ls;
+      }
+    }
+  }
+}
+
+// joins the splits of a row: one block per (b, key head, row), threads = columns
+template <typename T, int D, int MAPS>
+__global__ __launch_bounds__(D < 64 ? 64 : D) void attn_join_kernel(const Params p) {
+  const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
+  const int row = (int)blockIdx.x % rows, bk = (int)blockIdx.x / rows, hk = bk % p.Hkv, b = bk / p.Hkv;
+  const int d = threadIdx.x, g = row / p.Sq, qi = row % p.Sq, h = hk * G + g;
+  const float* part = p.part + ((size_t)bk * rblocks + row / 32) * p.splits * part_floats<D, MAPS>();
+  float o[MAPS];
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) {
+    const float* st = part + MAPS * 32 * D + (a * 32 + row % 32) * 2;
+    float mm = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, st[(size_t)s * part_floats<D, MAPS>()]);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f, l = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float f = exp2_(st[(size_t)s * part_floats<D, MAPS>()] - base);
+      l += f * st[(size_t)s * part_floats<D, MAPS>() + 1];
+      if (d < D) sum += f * part[(size_t)s * part_floats<D, MAPS>() + (a * 32 + row % 32) * D + d];
+    }
+    o[a] = l > 0.f ? sum / l : 0.f;
+    if (p.lse && d == 0) p.lse[(((size_t)b * p.H + h) * MAPS + a) * p.Sq + qi] = l > 0.f ? mm + __builtin_amdgcn_logf(l) : INFINITY;
+  }
+  if (d >= D) return;
+  const size_t at = (((size_t)b * p.Sq + qi) * p.H + h) * D + d;
+  if constexpr (MAPS == 2) {
+    if (p.out2) ((T*)p.out2)[at] = (T)o[1];
+    ((T*)p.out)[at] = (T)(o[0] - ldf(p.lam, h, p.lam_f32) * o[1]);
+  } else {
+    ((T*)p.out)[at] = (T)o[0];
+  }
+}
+
+constexpr int STEP_KEYS = 2 * TILE;      // keys of one round of a step-form block
+
+struct Plan {
+  bool step;
+  int splits, chunk, rblocks;
+  size_t lds, part_bytes;
+};
+
+template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
+  Plan r{};
+  const long long G = p.H / p.Hkv, rows = G * p.Sq;
+  const size_t bias = p.bk.n ? (size_t)((2 * p.bk.reach + 16) & ~15) + 4 * (size_t)p.bk.n * G : 0;
+  const size_t meet = (size_t)4 * 32 * (D + 4) * 4 + 4 * 32 * 2 * 4;
+  r.lds = 4 * (size_t)Tile<T, D>::BYTES + bias;
+  if (r.lds < meet) r.lds = meet;
+  r.step = rows <= 32 && r.lds <= 160 * 1024;
+  r.rblocks = (int)((rows + 31) / 32);
+  if (!r.step) return r;
+  const long long base = (long long)p.B * p.Hkv * r.rblocks, most = (p.Sk + STEP_KEYS - 1) / STEP_KEYS;
+  long long want = (1024 + base - 1) / base;
+  if (want > most) want = most;
+  r.chunk = (int)(((p.Sk + want - 1) / want + STEP_KEYS - 1) / STEP_KEYS * STEP_KEYS);
+  r.splits = (p.Sk + r.chunk - 1) / r.chunk;
+  r.part_bytes = (size_t)base * r.splits * part_floats<D, MAPS>() * 4;
+  return r;
+}
+
+template <typename T, int D, int MAPS> size_t fwd_workspace(const Params& p) { return plan_of<T, D, MAPS>(p).part_bytes; }
+
+template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t ws_bytes, hipStream_t st) {
+  const char* who = "token_attention_fwd";
+  const Plan r = plan_of<T, D, MAPS>(p);
+  if (r.step) {
+    EOVAE_CHECK_ARG(ws && ws_bytes >= r.part_bytes, "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, r.part_bytes);
+    p.part = (float*)ws;
+    p.splits = r.splits;
+    p.chunk = r.chunk;
+    const size_t base = (size_t)p.B * p.Hkv;
+    const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 256, r.lds, p, st, who);
+    if (rc) return rc;
+    return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, D < 64 ? 64 : D, 0, p, st, who);
+  }
+  constexpr int RB = 128 / MAPS;
+  size_t lds = 2 * (size_t)Tile<T, D>::BYTES + 4 * (size_t)bias_entries(p.bk);
+  if (MAPS == 2 && lds < (size_t)64 * (D + 4) * 4) lds = (size_t)64 * (D + 4) * 4;
+  return launch(attn_rows_kernel<T, D, MAPS>, (size_t)((p.Sq + RB - 1) / RB) * p.B * p.H, 256, lds, p, st, who);
+}
+
+}  // namespace
+
+extern "C" int eovae_token_attention_fwd(const eovae_token_attention* d, void* stream) {
+  Params p;
+  const int rc = make_params(d, p, "token_attention_fwd", 0);
+  if (rc) return rc;
+  return TOK_DISPATCH(d, run_fwd, p, d->ws, d->ws_bytes, (hipStream_t)stream);
+}
+
+size_t tok_fwd_workspace(const eovae_token_attention* d, const Params& p) { return TOK_DISPATCH(d, fwd_workspace, p); }

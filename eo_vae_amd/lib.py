@@ -16,6 +16,21 @@ _p, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 _ip = C.POINTER(C.c_int)
 _ll = C.c_longlong
 
+class TokenAttention(C.Structure):   # eovae_token_attention
+    _fields_ = ([(n, _p) for n in ('q', 'k', 'v', 'out', 'out2', 'lse', 'd_out', 'dq', 'dk', 'dv', 'dbias', 'dlam', 'bias', 'lam',
+                                   'kv_len', 'query_start', 'borders', 'ws')]
+                + [('ws_bytes', _sz), ('q_strides', _ll * 3), ('k_strides', _ll * 3), ('v_strides', _ll * 3)]
+                + [(n, _i) for n in ('dtype', 'bias_dtype', 'lam_dtype', 'maps', 'batch', 'sq', 'sk', 'heads', 'kv_heads', 'dim',
+                                     'start', 'causal', 'buckets', 'two_sided')] + [('scale', _f)])
+
+
+class TokenNorm(C.Structure):        # eovae_token_norm
+    _fields_ = ([(n, _p) for n in ('h', 'x', 'dy', 'dz', 'y', 'z', 'dh', 'dx', 'w1', 'b1', 'w2', 'b2', 'gate', 'dw1', 'db1', 'dw2',
+                                   'db2', 'dgate', 'stats', 'ws')]
+                + [('ws_bytes', _sz), ('rows', _ll), ('gates', _ll)]
+                + [(n, _i) for n in ('channels', 'layer', 'dtype', 'param_dtype')] + [('alpha', _f), ('eps', _f)])
+
+
 # name -> (restype, argtypes); mirrors include/eovae_hip.h one to one
 SIGNATURES = {
     'eovae_last_error': (C.c_char_p, []),
@@ -117,6 +132,12 @@ SIGNATURES = {
     'eovae_adam_step': (_i, [_p, _p, _p, _p, _sz, _f, _f, _f, _f, _i, _p, _f, _f, _p]),
     'eovae_scale_inplace': (_i, [_p, _sz, _p, _f, _p]),
     'eovae_multi_gather': (_i, [_p, _i, _p, _p]),
+    'eovae_token_attention_workspace': (_sz, [C.POINTER(TokenAttention), _i]),
+    'eovae_token_attention_fwd': (_i, [C.POINTER(TokenAttention), _p]),
+    'eovae_token_attention_bwd': (_i, [C.POINTER(TokenAttention), _p]),
+    'eovae_token_norm_workspace': (_sz, [C.POINTER(TokenNorm)]),
+    'eovae_token_norm_fwd': (_i, [C.POINTER(TokenNorm), _p]),
+    'eovae_token_norm_bwd': (_i, [C.POINTER(TokenNorm), _p]),
 }
 
 _lib = None

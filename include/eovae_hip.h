@@ -489,6 +489,69 @@ int eovae_resize_rot_bwd(const float* dy, float* dx, int planes, int Hs, int Ws,
 int eovae_area_rot(const float* src, float* dst, int planes, int Hs, int Ws, int Ht, int Wt, int rot,
                    void* stream);
 
+/* ----------------------------------------------------------------------------------------
+ * Token operators (csrc/token_attn_fwd.hip, token_attn_bwd.hip): fused attention over token rows with a learned relative
+ * position bias by buckets, one softmax map or the difference of two.
+ *   S_m = scale * q_m k_m^T + bias[bucket(key position - query position)][head]
+ *   out = softmax(S_0) v            maps = 1
+ *       = (softmax(S_0) - lam[head] softmax(S_1)) v     maps = 2: map m uses columns m * dim / 2 .. of q and k
+ * q [batch][sq][heads][dim], k and v [batch][sk][kv_heads][dim] by element strides {batch, token, head}, the last axis
+ * contiguous, 16-byte aligned; heads is a multiple of kv_heads (head h reads key head h / (heads / kv_heads)).  out, out2,
+ * d_out, dq contiguous [batch][sq][heads][dim]; dk, dv contiguous [batch][sk][kv_heads][dim].
+ * Key row j of sequence b is visible to query row i when j < kv_len[b] (NULL: sk) and, with causal, j <= query_start[b] + i
+ * (NULL: start + i).  Rows behind kv_len are never read.  A query that sees nothing gives zeros and no gradient.
+ * bias [buckets][heads] (NULL: none).  One side has n = buckets (two_sided: buckets / 2) of them: distance d < n / 2 is
+ * bucket d, then borders[i] (host memory, n - n / 2 - 1 ascending distances) is the first distance of bucket n / 2 + 1 + i;
+ * two_sided: keys ahead of the query use the second half of the table, else they count as distance 0.
+ * lse [batch][heads][maps][sq] (forward: nullable; the backward needs it), out2: the second map's own output (maps = 2; needed
+ * by the backward).  dbias [buckets][heads] and dlam [heads] are nullable and have the type of bias / lam.
+ * ws: eovae_token_attention_workspace(d, backward) bytes (d as for the call, ws aside); 0 where none is needed or the
+ * descriptor is refused.
+ * dtype, bias_dtype, lam_dtype: EOVAE_F32 or EOVAE_BF16.  All sums and statistics are fp32; gradients are bit-reproducible.
+ * -------------------------------------------------------------------------------------- */
+#define EOVAE_F32 0
+#define EOVAE_BF16 1
+typedef struct eovae_token_attention {
+  const void *q, *k, *v;
+  void *out, *out2;
+  float* lse;
+  const void* d_out;
+  void *dq, *dk, *dv, *dbias, *dlam;
+  const void *bias, *lam;
+  const int *kv_len, *query_start, *borders;
+  void* ws;
+  size_t ws_bytes;
+  long long q_strides[3], k_strides[3], v_strides[3];
+  int dtype, bias_dtype, lam_dtype, maps, batch, sq, sk, heads, kv_heads, dim, start, causal, buckets, two_sided;
+  float scale;
+} eovae_token_attention;
+size_t eovae_token_attention_workspace(const eovae_token_attention* d, int backward);
+int eovae_token_attention_fwd(const eovae_token_attention* d, void* stream);
+int eovae_token_attention_bwd(const eovae_token_attention* d, void* stream);
+
+/* Residual step of a token model (csrc/token_norm.hip):
+ *   y = alpha * x + gate * (norm(h) * w1 + b1)      z = norm(y) * w2 + b2
+ * h, x, y, z, dy, dz, dh, dx [rows][channels] contiguous in `dtype` (channels <= 8192); layer 1: LayerNorm, 0: root mean square
+ * (no biases).  gate [gates][channels], row r uses gate row r / (rows / gates); NULL with gates = 0: 1 everywhere.  z NULL
+ * (and w2, dz NULL): no second norm.  stats [rows][4] (mean, 1 / sigma of both norms): nullable forward, needed backward, which
+ * forms y again from h and x.  w1, b1, w2, b2, gate and their gradients (each nullable) have `param_dtype`.
+ * ws: eovae_token_norm_workspace(d) bytes for the backward (taken from rows, channels, gates and layer). */
+typedef struct eovae_token_norm {
+  const void *h, *x, *dy, *dz;
+  void *y, *z, *dh, *dx;
+  const void *w1, *b1, *w2, *b2, *gate;
+  void *dw1, *db1, *dw2, *db2, *dgate;
+  float* stats;
+  void* ws;
+  size_t ws_bytes;
+  long long rows, gates;
+  int channels, layer, dtype, param_dtype;
+  float alpha, eps;
+} eovae_token_norm;
+size_t eovae_token_norm_workspace(const eovae_token_norm* d);
+int eovae_token_norm_fwd(const eovae_token_norm* d, void* stream);
+int eovae_token_norm_bwd(const eovae_token_norm* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
