@@ -5,6 +5,12 @@
 //   dQ_m = scale dS_m K_m    dK_m = scale dS_m^T Q_m    dV = (sum_m w_m P_m)^T dO
 //   dbias[bucket] = sum of dS_0 (+ dS_1) over its pairs       dlambda = - sum dO o O_1
 //
+// delta comes from stored outputs, rounded to the tensors' type: good for dQ and dK, whose sums it enters with the mean of K
+// (of Q) only, but not for the two sums that it could drown.  The last buckets hold nearly all of a long row's probability, and
+// there sum dS = w (sum P dA - (mean of dA over the WHOLE row) (sum P)) is a difference of large values; lambda's gradient is
+// that mean.  Both are formed in fp32 from P and dA themselves, row by row; the mean is divided by the row's own sum of P, so that
+// a common error of P's scale (lse's rounding) cancels.
+//
 // attn_dq: a wave owns 32 queries and walks the keys; it also forms delta from O (for the second pass), the bias gradient's
 // partial sums (pairs of one distance lie on a diagonal of the score tile) and lambda's.  attn_dkv: a wave owns 32 keys and
 // walks the queries of every head that shares its key head, so shared heads' gradients are summed in a fixed order.  The
@@ -85,7 +91,11 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   const float c = p.scale * LOG2E;
-  float far_l = 0.f, far_r = 0.f;
+  // of this lane's query and map: sum P dA and sum P over the row, and over the keys of the two last buckets
+  float x[MAPS], m[MAPS], xl[MAPS], xr[MAPS], ml[MAPS], mr[MAPS], far_l = 0.f, far_r = 0.f;
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) x[a] = m[a] = xl[a] = xr[a] = ml[a] = mr[a] = 0.f;
+  const bool sums = p.part || p.lam_part;
   u32x4 rk[TK::PER], rv[TK::PER];
   if (kend > 0) {
     TK::fetch(rk, kb, p.ks, 0, limit, tid);
@@ -127,8 +137,21 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
           const int k = acc_row(r, half);
           float e = exp2_(s[r] * c + (tb ? tb[k] : far) - lse[a]);
           if (!whole && (key0 + k >= limit || (p.causal && key0 + k > qpos))) e = 0.f;
-          s[r] = e * ((a == 0 ? da[r] : -lam * da[r]) - delta[a]);
+          s[r] = e;
         }
+        if (sums) {
+          float xs = 0.f, ms = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            xs = fmaf(s[r], da[r], xs);
+            ms += s[r];
+          }
+          x[a] += xs, m[a] += ms;
+          if (side < 0) xl[a] += xs, ml[a] += ms;
+          if (side > 0) xr[a] += xs, mr[a] += ms;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= (a == 0 ? da[r] : -lam * da[r]) - delta[a];
         if (a == 0) both = s;
         else both += s;
 #pragma unroll
@@ -140,35 +163,36 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
             acc[a * (W / 32) + j] = mma(TK::frag_t(lk, 32 * t + 16 * u, a * W + 32 * j, lane), sf, acc[a * (W / 32) + j]);
         }
       }
-      if (p.part) {
-        if (side) {
-          float sum = 0.f;
+      if (p.part && !side) {
+        // rows = this wave's queries, columns = keys; then lane l sums diagonal key - query = l - 31 (63 of them)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += both[r];
-          if (side < 0) far_l += sum;
-          else far_r += sum;
-        } else {
-          // rows = this wave's queries, columns = keys; then lane l sums diagonal key - query = l - 31 (63 of them)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) scr[(lane & 31) * SCR + acc_row(r, half)] = both[r];
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const int off = lane - 31;
-          float sum = 0.f;
-          for (int q = 0; q < 32; ++q) {
-            const int k = q + off;
-            if (k >= 0 && k < 32) sum += scr[q * SCR + k];
-          }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const int rel = key0 - qlo + off;
-          if (off > 31) sum = 0.f;                                 // lane 63: no diagonal
-          if (rel <= -reach) far_l += sum;
-          else if (rel >= reach) far_r += sum;
-          else if (off <= 31) diag[rel + reach] += sum;             // one lane per distance
+        for (int r = 0; r < 16; ++r) scr[(lane & 31) * SCR + acc_row(r, half)] = both[r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int off = lane - 31;
+        float sum = 0.f;
+        for (int q = 0; q < 32; ++q) {
+          const int k = q + off;
+          if (k >= 0 && k < 32) sum += scr[q * SCR + k];
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int rel = key0 - qlo + off;
+        if (off > 31) sum = 0.f;                                   // lane 63: no diagonal
+        if (rel <= -reach) far_l += sum;
+        else if (rel >= reach) far_r += sum;
+        else if (off <= 31) diag[rel + reach] += sum;               // one lane per distance
       }
     }
+  }
+#pragma unroll
+  for (int a = 0; a < MAPS; ++a) {
+    x[a] += other_half(x[a]);
+    m[a] += other_half(m[a]);
+    x[a] = m[a] > 0.f ? x[a] / m[a] : 0.f;
+    const float w = a == 0 ? 1.f : -lam;
+    far_l += w * (xl[a] - x[a] * ml[a]);        // both halves: the sum over the wave adds their keys
+    far_r += w * (xr[a] - x[a] * mr[a]);
   }
   if (live) {
     T* dq = (T*)p.dq + orow;
@@ -212,9 +236,9 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
   }
   if constexpr (MAPS == 2) {
     if (p.lam_part) {
-      const float x = wave_sum(half == 0 && live ? d2 : 0.f);
+      const float xs = wave_sum(half == 0 ? x[1] : 0.f);
       __shared__ float lams[4];
-      if (lane == 0) lams[wave] = x;
+      if (lane == 0) lams[wave] = xs;
       __syncthreads();
       if (tid == 0) p.lam_part[slot] = -(lams[0] + lams[1] + lams[2] + lams[3]);
     }

@@ -22,11 +22,6 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MAX_BUCKETS, MAX_REACH, MAX_CHANNELS = 128, 1024, 8192
 
 
-def _need(cond, text):
-    if not cond:
-        raise ValueError(text)
-
-
 @functools.lru_cache(maxsize=64)
 def bucket_borders(side, max_distance):
     """First distance of every bucket behind the exact half of one side's `side` buckets: with e = side // 2 exact buckets and
@@ -44,33 +39,67 @@ def bucket_borders(side, max_distance):
     return tuple(out)
 
 
+@functools.lru_cache(maxsize=64)
+def _borders(side, max_distance):
+    """`bucket_borders` as the C array a descriptor points to; the cache keeps it alive."""
+    edge = bucket_borders(side, max_distance)
+    arr = (C.c_int * max(1, len(edge)))(*edge)
+    return C.addressof(arr), arr
+
+
 def _check_gpu(what, t, *others):
     if not t.is_cuda:
         raise L.EovaeError(f'{what}: tensor is on {t.device}; eo_vae_amd kernels only run on an AMD GPU (no CPU fallback) -- '
                            'move the model and inputs to "cuda"')
+    dev = t.device
     for o in others:
-        if o is not None and o.device != t.device:
-            raise L.EovaeError(f'{what}: tensors on {t.device} and {o.device}')
+        if o is not None and o.device != dev:
+            raise L.EovaeError(f'{what}: tensors on {dev} and {o.device}')
 
 
 def _rows16(t):
     """`t` itself where the kernels can read it as it lies (last axis contiguous, rows and address on 16 bytes), else a copy."""
     es = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+    st = t.stride()
+    if t.data_ptr() % 16 == 0 and st[3] == 1 and st[0] * es % 16 == 0 and st[1] * es % 16 == 0 and st[2] * es % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(t):
-    return (C.c_longlong * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+def _flat16(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _tracked(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _stream(t):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _like(t):
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+class _on:
+    """The tensor's device for the calls inside (no switch where it is the current one); yields its current stream."""
+
+    def __init__(self, t):
+        i = t.device.index
+        self.guard = None if i == torch.cuda.current_device() else torch.cuda.device(i)
+        self.index = i
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
 
 
 # ------------------------------------------------------------------------------------------
@@ -78,132 +107,127 @@ def _stream(t):
 # ------------------------------------------------------------------------------------------
 
 
-def _describe(q, k, v, bias, lam, kv_len, query_start, maps, two_sided, borders, causal, scale, start):
-    """The descriptor of a call; `borders` is a ctypes array that outlives it."""
-    d = L.TokenAttention()
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.q_strides, d.k_strides, d.v_strides = _strides(q), _strides(k), _strides(v)
-    d.batch, d.sq, d.heads, d.dim = q.shape
-    d.sk, d.kv_heads = k.shape[1], k.shape[2]
-    d.dtype, d.maps, d.causal, d.scale, d.start = _DTYPES[q.dtype], maps, int(causal), scale, start
-    if bias is not None:
-        d.bias, d.bias_dtype, d.buckets, d.two_sided = bias.data_ptr(), _DTYPES[bias.dtype], bias.shape[0], int(two_sided)
-        d.borders = C.cast(borders, C.c_void_p).value
-    if lam is not None:
-        d.lam, d.lam_dtype = lam.data_ptr(), _DTYPES[lam.dtype]
-    if kv_len is not None:
-        d.kv_len = kv_len.data_ptr()
-    if query_start is not None:
-        d.query_start = query_start.data_ptr()
-    return d
-
-
-def _call(fn, d, backward, t):
+def _launch_attention(fn, backward, device, stream, d):
     lib = L.load()
-    n = lib.eovae_token_attention_workspace(C.byref(d), backward)
-    ws = torch.empty(n, dtype=torch.uint8, device=t.device) if n else None
+    ref = C.byref(d)
+    n = lib.eovae_token_attention_workspace(ref, backward)
     if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
         d.ws, d.ws_bytes = ws.data_ptr(), n
-    L.check(getattr(lib, fn)(C.byref(d), _stream(t)), fn)
+    L.check(fn(ref, stream), 'token_attention_bwd' if backward else 'token_attention_fwd')
+
+
+def _describe(q, k, v, out, out2, lse, bias, lam, kv_len, query_start, rest, d_out=None, dq=None, dk=None, dv=None, dbias=None, dlam=None):
+    maps, two_sided, borders, causal, scale, start = rest
+    b, sq, h, dim = q.shape
+    return L.TokenAttention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out2), _ptr(lse), _ptr(d_out), _ptr(dq), _ptr(dk), _ptr(dv),
+        _ptr(dbias), _ptr(dlam), _ptr(bias), _ptr(lam), _ptr(kv_len), _ptr(query_start), borders, None, 0, q.stride()[:3], k.stride()[:3],
+        v.stride()[:3], _DTYPES[q.dtype], 0 if bias is None else _DTYPES[bias.dtype], 0 if lam is None else _DTYPES[lam.dtype], maps, b, sq,
+        k.shape[1], h, k.shape[2], dim, start, causal, 0 if bias is None else bias.shape[0], two_sided, scale)
+
+
+def _attention_forward(q, k, v, bias, lam, kv_len, query_start, keep, rest):
+    out = _like(q)
+    lse = out2 = None
+    if keep:
+        b, sq, h, _ = q.shape
+        lse = torch.empty((b, h, rest[0], sq), dtype=torch.float32, device=q.device)
+        if lam is not None:
+            out2 = _like(q)
+    with _on(q) as stream:
+        d = _describe(q, k, v, out, out2, lse, bias, lam, kv_len, query_start, rest)
+        _launch_attention(L.load().eovae_token_attention_fwd, 0, q.device, stream, d)
+    return out, out2, lse
 
 
 class TokenAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, lam, kv_len, query_start, keep, maps, two_sided, borders, causal, scale, start):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        bias = None if bias is None else bias.contiguous()
-        lam = None if lam is None else lam.contiguous()
-        b, sq, h, dim = q.shape
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        rest = (maps, two_sided, borders, causal, scale, start)
-        with torch.cuda.device(q.device):
-            d = _describe(q, k, v, bias, lam, kv_len, query_start, *rest)
-            d.out = out.data_ptr()
-            lse = out2 = None
-            if keep:
-                lse = torch.empty(b, h, maps, sq, dtype=torch.float32, device=q.device)
-                d.lse = lse.data_ptr()
-                if maps == 2:
-                    out2 = torch.empty_like(out)
-                    d.out2 = out2.data_ptr()
-            _call('eovae_token_attention_fwd', d, 0, q)
-        if keep:
-            ctx.save_for_backward(q, k, v, bias, lam, kv_len, query_start, out, out2, lse)
-            ctx.rest = rest
+    def forward(ctx, q, k, v, bias, lam, kv_len, query_start, rest):
+        out, out2, lse = _attention_forward(q, k, v, bias, lam, kv_len, query_start, True, rest)
+        ctx.save_for_backward(q, k, v, bias, lam, kv_len, query_start, out, out2, lse)
+        ctx.rest = rest
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         q, k, v, bias, lam, kv_len, query_start, out, out2, lse = ctx.saved_tensors
-        d_out = d_out.contiguous()
-        if d_out.data_ptr() % 16:
-            d_out = d_out.clone()
-        empty = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)   # noqa: E731
-        dq, dk, dv = empty(q), empty(k), empty(v)
-        dbias = empty(bias) if bias is not None and ctx.needs_input_grad[3] else None
-        dlam = empty(lam) if lam is not None and ctx.needs_input_grad[4] else None
-        with torch.cuda.device(q.device):
-            d = _describe(q, k, v, bias, lam, kv_len, query_start, *ctx.rest)
-            d.out, d.lse, d.d_out = out.data_ptr(), lse.data_ptr(), d_out.data_ptr()
-            d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-            if out2 is not None:
-                d.out2 = out2.data_ptr()
-            if dbias is not None:
-                d.dbias = dbias.data_ptr()
-            if dlam is not None:
-                d.dlam = dlam.data_ptr()
-            _call('eovae_token_attention_bwd', d, 1, q)
-        return (dq, dk, dv, dbias, dlam) + (None,) * 9
+        d_out = _flat16(d_out)
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        dbias = _like(bias) if bias is not None and ctx.needs_input_grad[3] else None
+        dlam = _like(lam) if lam is not None and ctx.needs_input_grad[4] else None
+        with _on(q) as stream:
+            d = _describe(_rows16(q), _rows16(k), _rows16(v), out, out2, lse, bias, lam, kv_len, query_start, ctx.rest, d_out, dq, dk, dv,
+                          dbias, dlam)
+            _launch_attention(L.load().eovae_token_attention_bwd, 1, q.device, stream, d)
+        return dq, dk, dv, dbias, dlam, None, None, None
 
 
 def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional, causal, scale, kv_len, query_start):
     for n, t in (('q', q), ('k', k), ('v', v)):
-        _need(t.dim() == 4, f'{what}: {n} has shape {tuple(t.shape)}, wants [batch, tokens, heads, width]')
-        _need(t.dtype in _DTYPES, f'{what}: {n} is {t.dtype} (float32 or bfloat16)')
-    _need(q.dtype == k.dtype == v.dtype, f'{what}: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}')
+        if not (t.dim() == 4):
+            raise ValueError(f'{what}: {n} has shape {tuple(t.shape)}, wants [batch, tokens, heads, width]')
+        if not (t.dtype in _DTYPES):
+            raise ValueError(f'{what}: {n} is {t.dtype} (float32 or bfloat16)')
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f'{what}: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}')
     b, sq, h, dim = q.shape
-    _need(k.shape == v.shape, f'{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ')
+    if not (k.shape == v.shape):
+        raise ValueError(f'{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ')
     sk, hk = k.shape[1], k.shape[2]
-    _need(k.shape[0] == b and k.shape[3] == dim, f'{what}: q {tuple(q.shape)} and k {tuple(k.shape)} disagree in batch or width')
-    _need(hk > 0 and h % hk == 0, f'{what}: {h} heads over {hk} key heads')
+    if not (k.shape[0] == b and k.shape[3] == dim):
+        raise ValueError(f'{what}: q {tuple(q.shape)} and k {tuple(k.shape)} disagree in batch or width')
+    if not (hk > 0 and h % hk == 0):
+        raise ValueError(f'{what}: {h} heads over {hk} key heads')
     widths = (32, 64, 128) if maps == 1 else (64, 128)
-    _need(dim in widths, f'{what}: head width {dim}, wants one of {widths}')
-    _need(max(sq, sk) <= 1 << 28, f'{what}: {sq} queries, {sk} keys (at most 2^28)')
+    if not (dim in widths):
+        raise ValueError(f'{what}: head width {dim}, wants one of {widths}')
+    if not (max(sq, sk) <= 1 << 28):
+        raise ValueError(f'{what}: {sq} queries, {sk} keys (at most 2^28)')
     two_sided, borders = False, None
     if bias_table is not None:
-        _need(bias_table.dim() == 2 and bias_table.shape[1] == h, f'{what}: bias_table {tuple(bias_table.shape)}, wants [buckets, {h}]')
-        _need(bias_table.dtype in _DTYPES, f'{what}: bias_table is {bias_table.dtype} (float32 or bfloat16)')
+        if not (bias_table.dim() == 2 and bias_table.shape[1] == h):
+            raise ValueError(f'{what}: bias_table {tuple(bias_table.shape)}, wants [buckets, {h}]')
+        if not (bias_table.dtype in _DTYPES):
+            raise ValueError(f'{what}: bias_table is {bias_table.dtype} (float32 or bfloat16)')
         two_sided = bool(bidirectional)
         n = bias_table.shape[0]
         side = n // 2 if two_sided else n
-        _need(side >= 2 and n <= MAX_BUCKETS and not (two_sided and n % 2),
-              f'{what}: {n} buckets; wants 2 .. {MAX_BUCKETS}, bidirectional an even number of at least 4')
-        _need(side // 2 < max_distance <= MAX_REACH, f'{what}: max_distance {max_distance}, wants {side // 2} < max_distance <= {MAX_REACH}')
-        edge = bucket_borders(side, int(max_distance))
-        borders = (C.c_int * max(1, len(edge)))(*edge)
+        if not (side >= 2 and n <= MAX_BUCKETS and not (two_sided and n % 2)):
+            raise ValueError(f'{what}: {n} buckets; wants 2 .. {MAX_BUCKETS}, bidirectional an even number of at least 4')
+        if not (side // 2 < max_distance <= MAX_REACH):
+            raise ValueError(f'{what}: max_distance {max_distance}, wants {side // 2} < max_distance <= {MAX_REACH}')
+        borders = _borders(side, int(max_distance))[0]
+        bias_table = bias_table.contiguous()
     if lam is not None:
-        _need(lam.shape == (h,), f'{what}: lam has shape {tuple(lam.shape)}, wants [{h}]')
-        _need(lam.dtype in _DTYPES, f'{what}: lam is {lam.dtype} (float32 or bfloat16)')
+        if not (lam.shape == (h,)):
+            raise ValueError(f'{what}: lam has shape {tuple(lam.shape)}, wants [{h}]')
+        if not (lam.dtype in _DTYPES):
+            raise ValueError(f'{what}: lam is {lam.dtype} (float32 or bfloat16)')
     start = sk - sq
     if isinstance(query_start, int) and not isinstance(query_start, bool):
-        _need(abs(query_start) <= 1 << 30, f'{what}: query_start {query_start} (at most 2^30 either way)')
+        if not (abs(query_start) <= 1 << 30):
+            raise ValueError(f'{what}: query_start {query_start} (at most 2^30 either way)')
         start, query_start = query_start, None
     elif query_start is None:
-        _need(kv_len is None or not (causal or bias_table is not None),
-              f'{what}: kv_len with causal or a bias needs query_start (the position of the first query among the keys)')
+        if not (kv_len is None or not (causal or bias_table is not None)):
+            raise ValueError(f'{what}: kv_len with causal or a bias needs query_start (the position of the first query among the keys)')
     for n, t in (('kv_len', kv_len), ('query_start', query_start)):
         if t is not None:
-            _need(torch.is_tensor(t) and t.dtype == torch.int32 and t.shape == (b,) and t.is_contiguous(),
-                  f'{what}: {n} wants a contiguous int32 tensor [{b}]' + (' or an int' if n == 'query_start' else ''))
+            if not (torch.is_tensor(t) and t.dtype == torch.int32 and t.shape == (b,) and t.is_contiguous()):
+                raise ValueError(f'{what}: {n} wants a contiguous int32 tensor [{b}]' + (' or an int' if n == 'query_start' else ''))
     _check_gpu(what, q, k, v, lam, bias_table, kv_len, query_start)
     if scale is None:
         scale = float(dim // maps) ** -0.5
     if q.numel() == 0 or sk == 0:      # nothing to attend to: zeros, tied to the inputs so that gradients are zeros too
         zero = v.sum() * 0 + (0 if lam is None else lam.sum() * 0) + (0 if bias_table is None else bias_table.sum() * 0) + k.sum() * 0
         return q * 0 + zero.to(q.dtype)
-    return TokenAttentionFn.apply(q, k, v, bias_table, lam, kv_len, query_start, _tracked(q, k, v, bias_table, lam), maps, two_sided, borders,
-                                  bool(causal), float(scale), start)
+    args = (_rows16(q), _rows16(k), _rows16(v), bias_table, None if lam is None else lam.contiguous(), kv_len, query_start)
+    rest = (maps, two_sided, borders, bool(causal), float(scale), start)
+    if _tracked(q, k, v, bias_table, lam):
+        return TokenAttentionFn.apply(*args, rest)
+    return _attention_forward(*args, False, rest)[0]
 
 
 def rel_pos_attention(q, k, v, bias_table=None, *, max_distance=128, bidirectional=True, causal=False, scale=None, kv_len=None,
@@ -231,7 +255,8 @@ def diff_attention(q, k, v, lam, bias_table=None, *, max_distance=128, bidirecti
 
     q0, q1 (k0, k1) are the halves of the last axis of q (k): width 64 or 128, maps of 32 or 64 columns over values of the
     whole width; scale: (width / 2)^-0.5.  lam [heads], learned; everything else as in `rel_pos_attention`."""
-    _need(torch.is_tensor(lam), 'diff_attention: lam wants a tensor [heads]')
+    if not (torch.is_tensor(lam)):
+        raise ValueError('diff_attention: lam wants a tensor [heads]')
     return _attention('diff_attention', 2, q, k, v, lam, bias_table, max_distance, bidirectional, causal, scale, kv_len, query_start)
 
 
@@ -240,38 +265,32 @@ def diff_attention(q, k, v, lam, bias_table=None, *, max_distance=128, bidirecti
 # ------------------------------------------------------------------------------------------
 
 
-def _norm_desc(h, x, w1, b1, w2, b2, gate, layer, alpha, eps):
-    d = L.TokenNorm()
-    for n, t in (('h', h), ('x', x), ('w1', w1), ('b1', b1), ('w2', w2), ('b2', b2), ('gate', gate)):
-        if t is not None:
-            setattr(d, n, t.data_ptr())
-    d.channels = h.shape[-1]
-    d.rows = h.numel() // d.channels
-    d.gates = 0 if gate is None else gate.numel() // d.channels
-    d.layer, d.dtype, d.param_dtype, d.alpha, d.eps = int(layer), _DTYPES[h.dtype], _DTYPES[w1.dtype], alpha, eps
-    return d
+def _describe_norm(h, x, w1, b1, w2, b2, gate, stats, rest, y=None, z=None, dy=None, dz=None, dh=None, dx=None, grads=(None,) * 5):
+    layer, alpha, eps = rest
+    c = h.shape[-1]
+    dw1, db1, dw2, db2, dgate = grads
+    return L.TokenNorm(
+        h.data_ptr(), x.data_ptr(), _ptr(dy), _ptr(dz), _ptr(y), _ptr(z), _ptr(dh), _ptr(dx), w1.data_ptr(), _ptr(b1), _ptr(w2), _ptr(b2),
+        _ptr(gate), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), _ptr(dgate), _ptr(stats), None, 0, h.numel() // c,
+        0 if gate is None else gate.numel() // c, c, layer, _DTYPES[h.dtype], _DTYPES[w1.dtype], alpha, eps)
+
+
+def _norm_forward(h, x, w1, b1, w2, b2, gate, keep, rest):
+    y = _like(h)
+    z = _like(h) if w2 is not None else None
+    stats = torch.empty((h.numel() // h.shape[-1], 4), dtype=torch.float32, device=h.device) if keep else None
+    with _on(h) as stream:
+        d = _describe_norm(h, x, w1, b1, w2, b2, gate, stats, rest, y, z)
+        L.check(L.load().eovae_token_norm_fwd(C.byref(d), stream), 'token_norm_fwd')
+    return y, z, stats
 
 
 class GatedNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, x, w1, b1, w2, b2, gate, keep, layer, alpha, eps):
-        h, x = h.contiguous(), x.contiguous()
-        w1, b1, w2, b2, gate = (None if t is None else t.contiguous() for t in (w1, b1, w2, b2, gate))
-        y = torch.empty_like(h)
-        z = torch.empty_like(h) if w2 is not None else None
-        with torch.cuda.device(h.device):
-            d = _norm_desc(h, x, w1, b1, w2, b2, gate, layer, alpha, eps)
-            d.y = y.data_ptr()
-            if z is not None:
-                d.z = z.data_ptr()
-            stats = None
-            if keep:
-                stats = torch.empty(d.rows, 4, dtype=torch.float32, device=h.device)
-                d.stats = stats.data_ptr()
-            L.check(L.load().eovae_token_norm_fwd(C.byref(d), _stream(h)), 'eovae_token_norm_fwd')
-        if keep:
-            ctx.save_for_backward(h, x, w1, b1, w2, b2, gate, stats)
-            ctx.rest = (layer, alpha, eps)
+    def forward(ctx, h, x, w1, b1, w2, b2, gate, rest):
+        y, z, stats = _norm_forward(h, x, w1, b1, w2, b2, gate, True, rest)
+        ctx.save_for_backward(h, x, w1, b1, w2, b2, gate, stats)
+        ctx.rest = rest
         ctx.set_materialize_grads(False)
         return (y, z) if z is not None else y
 
@@ -279,26 +298,20 @@ class GatedNormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dz=None):
         if dy is None and dz is None:
-            return (None,) * 11
+            return (None,) * 8
         h, x, w1, b1, w2, b2, gate, stats = ctx.saved_tensors
         dy = torch.zeros_like(h) if dy is None else dy.contiguous()
         dz = None if dz is None else dz.contiguous()
-        dh, dx = torch.empty_like(h), torch.empty_like(x)
-        grads = [None if t is None else torch.empty_like(t) for t in (w1, b1, w2, b2, gate)]
-        with torch.cuda.device(h.device):
-            d = _norm_desc(h, x, w1, b1, w2, b2, gate, *ctx.rest)
-            d.dy, d.dh, d.dx, d.stats = dy.data_ptr(), dh.data_ptr(), dx.data_ptr(), stats.data_ptr()
-            if dz is not None:
-                d.dz = dz.data_ptr()
-            for n, t in zip(('dw1', 'db1', 'dw2', 'db2', 'dgate'), grads):
-                if t is not None:
-                    setattr(d, n, t.data_ptr())
-            lib = L.load()
-            n = lib.eovae_token_norm_workspace(C.byref(d))
+        dh, dx = _like(h), _like(x)
+        grads = [None if t is None else _like(t) for t in (w1, b1, w2, b2, gate)]
+        with _on(h) as stream:
+            d = _describe_norm(h, x, w1, b1, w2, b2, gate, stats, ctx.rest, None, None, dy, dz, dh, dx, grads)
+            lib, ref = L.load(), C.byref(d)
+            n = lib.eovae_token_norm_workspace(ref)
             ws = torch.empty(n, dtype=torch.uint8, device=h.device)
             d.ws, d.ws_bytes = ws.data_ptr(), n
-            L.check(lib.eovae_token_norm_bwd(C.byref(d), _stream(h)), 'eovae_token_norm_bwd')
-        return (dh, dx, *grads, None, None, None, None)
+            L.check(lib.eovae_token_norm_bwd(ref, stream), 'token_norm_bwd')
+        return (dh, dx, *grads, None)
 
 
 def gated_norm_residual(h, x, post_weight, gate=None, pre_weight=None, *, post_bias=None, pre_bias=None, norm='rms', residual_scale=1.0,
@@ -310,31 +323,43 @@ def gated_norm_residual(h, x, post_weight, gate=None, pre_weight=None, *, post_b
     ones behind its leading axes ([batch, 1, channels]: a gate per sample).  Weights, biases and gate share one type, float32
     or that of h.  z is formed from the unrounded y."""
     what = 'gated_norm_residual'
-    _need(h.dtype in _DTYPES, f'{what}: h is {h.dtype} (float32 or bfloat16)')
-    _need(h.dim() >= 1 and x.shape == h.shape and x.dtype == h.dtype, f'{what}: h {tuple(h.shape)} {h.dtype} and x {tuple(x.shape)} {x.dtype} differ')
+    if not (h.dtype in _DTYPES):
+        raise ValueError(f'{what}: h is {h.dtype} (float32 or bfloat16)')
+    if not (h.dim() >= 1 and x.shape == h.shape and x.dtype == h.dtype):
+        raise ValueError(f'{what}: h {tuple(h.shape)} {h.dtype} and x {tuple(x.shape)} {x.dtype} differ')
     c = h.shape[-1]
-    _need(1 <= c <= MAX_CHANNELS, f'{what}: {c} channels (1 .. {MAX_CHANNELS})')
-    _need(norm in ('rms', 'layer'), f"{what}: norm {norm!r} ('rms' or 'layer')")
-    _need(norm == 'layer' or (post_bias is None and pre_bias is None), f'{what}: a root-mean-square norm has no bias')
-    _need(pre_weight is not None or pre_bias is None, f'{what}: pre_bias without pre_weight')
-    _need(post_weight.dtype in (torch.float32, h.dtype), f'{what}: post_weight is {post_weight.dtype} (float32 or {h.dtype})')
+    if not (1 <= c <= MAX_CHANNELS):
+        raise ValueError(f'{what}: {c} channels (1 .. {MAX_CHANNELS})')
+    if not (norm in ('rms', 'layer')):
+        raise ValueError(f"{what}: norm {norm!r} ('rms' or 'layer')")
+    if not (norm == 'layer' or (post_bias is None and pre_bias is None)):
+        raise ValueError(f'{what}: a root-mean-square norm has no bias')
+    if not (pre_weight is not None or pre_bias is None):
+        raise ValueError(f'{what}: pre_bias without pre_weight')
+    if not (post_weight.dtype in (torch.float32, h.dtype)):
+        raise ValueError(f'{what}: post_weight is {post_weight.dtype} (float32 or {h.dtype})')
     for n, t in (('post_weight', post_weight), ('post_bias', post_bias), ('pre_weight', pre_weight), ('pre_bias', pre_bias)):
-        _need(t is None or (t.shape == (c,) and t.dtype == post_weight.dtype), f'{what}: {n} wants {post_weight.dtype} [{c}]')
+        if not (t is None or (t.shape == (c,) and t.dtype == post_weight.dtype)):
+            raise ValueError(f'{what}: {n} wants {post_weight.dtype} [{c}]')
     if gate is not None:
         lead = tuple(gate.shape[:-1])
         k = len(lead)
         while k and lead[k - 1] == 1:
             k -= 1
-        _need(gate.dtype == post_weight.dtype, f'{what}: gate is {gate.dtype}, the weights {post_weight.dtype}')
-        _need(gate.dim() >= 1 and gate.shape[-1] == c and (gate.dim() == 1 or gate.dim() == h.dim()) and lead[:k] == tuple(h.shape[:k]),
-              f'{what}: gate {tuple(gate.shape)} for h {tuple(h.shape)}: [channels], or the shape of h with ones behind its leading axes')
-    _need(float(eps) > 0, f'{what}: eps {eps}')
+        if not (gate.dtype == post_weight.dtype):
+            raise ValueError(f'{what}: gate is {gate.dtype}, the weights {post_weight.dtype}')
+        if not (gate.dim() >= 1 and gate.shape[-1] == c and (gate.dim() == 1 or gate.dim() == h.dim()) and lead[:k] == tuple(h.shape[:k])):
+            raise ValueError(f'{what}: gate {tuple(gate.shape)} for h {tuple(h.shape)}: [channels], or the shape of h with ones behind its leading axes')
+    if not (float(eps) > 0):
+        raise ValueError(f'{what}: eps {eps}')
     _check_gpu(what, h, x, post_weight, post_bias, pre_weight, pre_bias, gate)
     if h.numel() == 0:
         tie = sum(t.sum() * 0 for t in (post_weight, post_bias, pre_weight, pre_bias, gate) if t is not None)
         y = residual_scale * x + h * 0 + tie.to(h.dtype)
         return y, (None if pre_weight is None else y * 1)
-    got = GatedNormFn.apply(h, x, post_weight, post_bias, pre_weight, pre_bias, gate,
-                            _tracked(h, x, post_weight, post_bias, pre_weight, pre_bias, gate), norm == 'layer', float(residual_scale),
-                            float(eps))
+    args = [None if t is None else t.contiguous() for t in (h, x, post_weight, post_bias, pre_weight, pre_bias, gate)]
+    rest = (norm == 'layer', float(residual_scale), float(eps))
+    if not _tracked(*args):
+        return _norm_forward(*args, False, rest)[:2]
+    got = GatedNormFn.apply(*args, rest)
     return got if pre_weight is not None else (got, None)
