@@ -71,8 +71,8 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
       for (int e = 0; e < 8; ++e) d1 += (float)gf[i].x[e] * (float)of.x[e];
     }
   }
-  d1 += other_half(d1);
-  d2 += other_half(d2);
+  d1 = column_sum(d1);
+  d2 = column_sum(d2);
   float lse[MAPS], delta[MAPS];
   delta[0] = d1;
   if constexpr (MAPS == 2) delta[1] = -lam * d2;
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
   }
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
-    x[a] += other_half(x[a]);
-    m[a] += other_half(m[a]);
+    x[a] = column_sum(x[a]);
+    m[a] = column_sum(m[a]);
     x[a] = m[a] > 0.f ? x[a] / m[a] : 0.f;
     const float w = a == 0 ? 1.f : -lam;
     far_l += w * (xl[a] - x[a] * ml[a]);        // both halves: the sum over the wave adds their keys

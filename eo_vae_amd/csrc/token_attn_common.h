@@ -186,8 +186,16 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
-// the value of the other half's lane with the same column
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// a column's two halves (lanes l and l + 32) together: v_permlane32_swap hands every lane both values
+struct Halves { float lo, hi; };
+__device__ __forceinline__ Halves halves(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned a = r[0], b = r[1];
+  return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+__device__ __forceinline__ float column_sum(float x) { const Halves h = halves(x); return h.lo + h.hi; }
+__device__ __forceinline__ float column_max(float x) { const Halves h = halves(x); return fmaxf(h.lo, h.hi); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ int key_limit(const Params& p, int b) {

@@ -14,60 +14,92 @@ using namespace tok;
 
 namespace {
 
-// One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
-// key0: position of the tile's first key; qpos: this lane's query position; limit: keys visible at all.
-template <typename T, int D, int W, int NT>
-__device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
-                                          float& m, float& l, int map, int key0, int lkey0, int limit, int qpos, int qlo, int qhi,
-                                          const float* tab, int lane) {
-  using TK = Tile<T, D>;
-  const int half = lane >> 5;
-  const float c = p.scale * LOG2E;
-  f32x16 s[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    s[t] = zero16();
-#pragma unroll
-    for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, lkey0 + 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
-  }
-  const int klast = key0 + 32 * NT - 1;
+// Scores of one wave's 32 queries against 32 NT keys, turned into probabilities in place (relative to 2^m, not normalised);
+// returns the factor by which the wave's earlier sums have to be multiplied (`moved`: whether any lane's differs from 1).
+// The reference m of a row is its maximum when it last moved: it follows only when a score passes it by 2^SLACK, which the
+// fp32 sums hold easily and which saves rescaling the output tile for almost every key tile.
+// Plain tiles (all pairs visible, one bias value) cost one fma and one exp2 per score; the others add bias and mask first.
+constexpr float SLACK = 8.f;
+template <int NT>
+__device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], float& m, float& l, bool& moved, float c, int key0, int limit,
+                                              int qpos, int qlo, int qhi, const float* tab, int lane) {
+  const int half = lane >> 5, klast = key0 + 32 * NT - 1;
   const bool whole = klast < limit && (!p.causal || klast <= qlo);
-  float top = -INFINITY;
-  const float* tb = nullptr;
   float far = 0.f;
+  bool near = false;
   if (p.bk.n) {
     const int reach = p.bk.reach;
     if (klast - qlo <= -reach) far = tab[PAD];                              // every pair at or behind the last border
     else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)];
-    else tb = tab + (reach + PAD) + key0 - qpos;
+    else near = true;
   }
+  if (near || !whole) {
+    const float* tb = tab + (p.bk.reach + PAD) + key0 - qpos + 4 * half;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int k = 32 * t + 8 * (r >> 2) + (r & 3);
+        s[t][r] = fmaf(s[t][r], c, near ? tb[k] : far);
+      }
+    if (!whole) {
+      // last visible key of this lane's query, relative to its first score
+      const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * t + 8 * (r >> 2) + (r & 3) > last) s[t][r] = -INFINITY;
+    }
+    c = 1.f;
+    far = 0.f;
+  }
+  float top = s[0][0];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int k = 32 * t + acc_row(r, half);
-      float x = s[t][r] * c + (tb ? tb[k] : far);
-      if (!whole && (key0 + k >= limit || (p.causal && key0 + k > qpos))) x = -INFINITY;
-      s[t][r] = x;
-      top = fmaxf(top, x);
-    }
-  top = fmaxf(top, other_half(top));
-  const float mn = fmaxf(m, top);
-  const float base = mn == -INFINITY ? 0.f : mn;
-  const float a = exp2_(m - base);                                        // m = -inf: 0
-  m = mn;
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+  top = fmaf(column_max(top), c, far);
+  float a = 1.f;
+  moved = __any(top > m + SLACK);
+  if (moved) {
+    const float mn = fmaxf(m, top);
+    a = exp2_(m - (mn == -INFINITY ? 0.f : mn));                             // m = -inf: 0
+    m = mn;
+    l *= a;
+  }
+  const float off = far - (m == -INFINITY ? 0.f : m);
   float sum = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float e = exp2_(s[t][r] - base);
-      s[t][r] = e;
-      sum += e;
+      s[t][r] = exp2_(fmaf(s[t][r], c, off));
+      sum += s[t][r];
     }
-  l = l * a + sum;
+  l += sum;
+  return a;
+}
+
+// One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
+// key0: position of the tile's first key; qpos: this lane's query position; limit: keys visible at all.
+template <typename T, int D, int W, int NT>
+__device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
+                                          float& m, float& l, float c, int map, int key0, int limit, int qpos, int qlo, int qhi, const float* tab,
+                                          int lane) {
+  using TK = Tile<T, D>;
+  f32x16 s[NT];
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) acc[j] *= a;
+  for (int t = 0; t < NT; ++t) {
+    s[t] = zero16();
+#pragma unroll
+    for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
+  }
+  bool moved;
+  const float a = softmax_tile<NT>(p, s, m, l, moved, c, key0, limit, qpos, qlo, qhi, tab, lane);
+  if (moved)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[j] *= a;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -75,12 +107,22 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
       Frag<T> pf;
       to_frag(pf, s[t], 8 * u);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) acc[j] = mma(TK::frag_t(lv, lkey0 + 32 * t + 16 * u, 32 * j, lane), pf, acc[j]);
+      for (int j = 0; j < D / 32; ++j) acc[j] = mma(TK::frag_t(lv, 32 * t + 16 * u, 32 * j, lane), pf, acc[j]);
     }
 }
 
+// a negative scale is carried by the queries, so that the largest product is the largest score
+template <typename T, int N> __device__ __forceinline__ float positive_scale(float scale, Frag<T> (&qf)[N]) {
+  if (scale < 0.f)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[i].x[e] = -qf[i].x[e];
+  return fabsf(scale) * LOG2E;
+}
+
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256) void attn_rows_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;                 // width of one map's queries and keys
   constexpr int RB = 128 / MAPS;              // query rows of a block
@@ -106,6 +148,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Params p) {
   Frag<T> qf[W / 16];
 #pragma unroll
   for (int i = 0; i < W / 16; ++i) qf[i] = frag_global(qp, i, lane, live);
+  const float c = positive_scale(p.scale, qf);
   if (p.bk.n) fill_bias(p, tab, h, tid, 256);
   f32x16 acc[D / 32];
 #pragma unroll
@@ -126,9 +169,9 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Params p) {
       TK::fetch(rv, vb, p.vs, k0 + TILE, limit, tid);
     }
     if (!p.causal || k0 <= qhi)
-      tile_step<T, D, W, 2>(p, lk, lv, qf, acc, m, l, map, k0, 0, limit, qpos, qlo, qhi, tab, lane);
+      tile_step<T, D, W, 2>(p, lk, lv, qf, acc, m, l, c, map, k0, limit, qpos, qlo, qhi, tab, lane);
   }
-  l += other_half(l);
+  l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] *= inv;
@@ -221,7 +264,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[a][i] = zero16();
   }
-  const float c = p.scale * LOG2E;
+  const float c = positive_scale(p.scale, qf);
   u32x4 rk[2][TK::PER], rv[2][TK::PER];
   if (k_lo < k_hi)
 #pragma unroll
@@ -266,7 +309,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
         s[r] = x;
         top = fmaxf(top, x);
       }
-      top = fmaxf(top, other_half(top));
+      top = column_max(top);
       const float mn = fmaxf(m[a], top), base = mn == -INFINITY ? 0.f : mn, al = exp2_(m[a] - base);
       m[a] = mn;
       float sum = 0.f;
@@ -295,7 +338,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
     __syncthreads();
-    const float lt = l[a] + other_half(l[a]);
+    const float lt = column_sum(l[a]);
     const int col = lane & 31;
     if (half == 0) {
       stat[(wave * 32 + col) * 2] = m[a];
