@@ -26,7 +26,7 @@ namespace {
 constexpr int SCR = TILE / 2 + 1;         // scratch row of a wave's 32 x 32 score-gradient tile (+ 1: diagonals spread over the banks)
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -115,13 +115,14 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
       const int key0 = k0 + 32 * t, klast = key0 + 31;
       if (key0 >= kend || (p.causal && key0 > qhi)) continue;
       const bool whole = klast < limit && (!p.causal || klast <= qlo);
-      const float* tb = nullptr;
+      const float* tb = tab + (reach + PAD) + key0 - qpos + 4 * half;
       float far = 0.f;
       int side = 0;
+      bool near = false;
       if (p.bk.n) {
         if (klast - qlo <= -reach) far = tab[PAD], side = -1;
         else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
-        else tb = tab + (reach + PAD) + key0 - qpos;
+        else near = true;
       }
       f32x16 da = zero16();
 #pragma unroll
@@ -132,13 +133,21 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
         f32x16 s = zero16();
 #pragma unroll
         for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lk, 32 * t, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
+        float cc = c, off = far - lse[a];
+        if (near || !whole) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int k = acc_row(r, half);
-          float e = exp2_(s[r] * c + (tb ? tb[k] : far) - lse[a]);
-          if (!whole && (key0 + k >= limit || (p.causal && key0 + k > qpos))) e = 0.f;
-          s[r] = e;
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, near ? tb[8 * (r >> 2) + (r & 3)] : far);
+          if (!whole) {
+            const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (8 * (r >> 2) + (r & 3) > last) s[r] = -INFINITY;
+          }
+          cc = 1.f;
+          off = -lse[a];
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], cc, off));
         if (sums) {
           float xs = 0.f, ms = 0.f;
 #pragma unroll
@@ -246,12 +255,12 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const Params p) {
 }
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_dkv_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char *lq = lds, *lg = lds + TK::BYTES;
-  float* rows = (float*)(lds + 2 * TK::BYTES);                    // [MAPS][2][TILE]: lse, delta
+  float* rows = (float*)(lds + 2 * TK::BYTES);                    // [MAPS][2][TILE]: -lse, delta
   float* tab = rows + MAPS * 2 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
@@ -301,7 +310,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const Params p) {
     if (tid < TILE)
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
-        rows[a * 2 * TILE + tid] = rl[a];
+        rows[a * 2 * TILE + tid] = -rl[a];
         rows[a * 2 * TILE + TILE + tid] = rd[a];
       }
     if (it % per == 0) {
@@ -315,12 +324,13 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const Params p) {
       const int r0 = q0 + 32 * t, qlo = start + r0, qhi = qlo + 31;
       if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
       const bool whole = khi < limit && (!p.causal || khi <= qlo);
-      const float* tb = nullptr;
+      const float* tb = tab + (reach + PAD) + krow - qlo - 4 * half;
       float far = 0.f;
+      bool near = false;
       if (p.bk.n) {
         if (khi - qlo <= -reach) far = tab[PAD];
         else if (klo - qhi >= reach) far = tab[2 * (reach + PAD)];
-        else tb = tab + (reach + PAD) + krow - qlo;
+        else near = true;
       }
       f32x16 da = zero16(), mix;
 #pragma unroll
@@ -331,14 +341,29 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const Params p) {
 #pragma unroll
         for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lq, 32 * t, a * (W / 16) + i, lane), kf[a * (W / 16) + i], s);
         const float* ls = rows + a * 2 * TILE + 32 * t;
+        float cc = c;
+        if (near || !whole || far != 0.f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int q = acc_row(r, half);
-          float e = exp2_(s[r] * c + (tb ? tb[-q] : far) - ls[q]);
-          if (!whole && (krow >= limit || (p.causal && krow > qlo + q))) e = 0.f;
-          if (a == 0) mix[r] = e;
-          else mix[r] -= lam * e;
-          s[r] = e * ((a == 0 ? da[r] : -lam * da[r]) - ls[TILE + q]);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, near ? tb[-(8 * (r >> 2) + (r & 3))] : far);
+          if (!whole) {
+            const int first = krow >= limit ? 64 : (p.causal ? krow - qlo - 4 * half : 0);       // first query that sees this key
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (8 * (r >> 2) + (r & 3) < first) s[r] = -INFINITY;
+          }
+          cc = 1.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 nl = *(const f32x4*)(ls + 8 * g + 4 * half), dl = *(const f32x4*)(ls + TILE + 8 * g + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            const float x = exp2_(fmaf(s[r], cc, nl[e]));
+            if (a == 0) mix[r] = x;
+            else mix[r] = fmaf(-lam, x, mix[r]);
+            s[r] = x * ((a == 0 ? da[r] : -lam * da[r]) - dl[e]);
+          }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
