@@ -23,15 +23,14 @@ using namespace tok;
 
 namespace {
 
-constexpr int SCR = TILE / 2 + 1;         // scratch row of a wave's 32 x 32 score-gradient tile (+ 1: diagonals spread over the banks)
+constexpr int SCR = 33;         // scratch row of a wave's 32 x 32 score-gradient tile (+ 1: diagonals spread over the banks)
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dq_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *lk = lds, *lv = lds + TK::BYTES;
-  float* tab = (float*)(lds + 2 * TK::BYTES);
+  float* tab = (float*)(lds + Stream<T, D>::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach, ndiag = 2 * reach + 1;
   float* diag = tab + ntab + wave * ndiag;                       // [4][2 reach + 1]: sums by distance, |distance| < reach used
@@ -96,22 +95,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) x[a] = m[a] = xl[a] = xr[a] = ml[a] = mr[a] = 0.f;
   const bool sums = p.part || p.lam_part;
-  u32x4 rk[TK::PER], rv[TK::PER];
-  if (kend > 0) {
-    TK::fetch(rk, kb, p.ks, 0, limit, tid);
-    TK::fetch(rv, vb, p.vs, 0, limit, tid);
-  }
-  for (int k0 = 0; k0 < kend; k0 += TILE) {
-    __syncthreads();
-    TK::put(lk, rk, tid);
-    TK::put(lv, rv, tid);
-    __syncthreads();
-    if (k0 + TILE < kend) {
-      TK::fetch(rk, kb, p.ks, k0 + TILE, limit, tid);
-      TK::fetch(rv, vb, p.vs, k0 + TILE, limit, tid);
-    }
+  Stream<T, D> kv(lds);
+  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
+  for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
+    kv.arrive();
+    if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, limit, tid);
+    char *lk = kv.a(), *lv = kv.b();
 #pragma unroll 1
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TK::ROWS / 32; ++t) {
       const int key0 = k0 + 32 * t, klast = key0 + 31;
       if (key0 >= kend || (p.causal && key0 > qhi)) continue;
       const bool whole = klast < limit && (!p.causal || klast <= qlo);
@@ -127,7 +118,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
       f32x16 da = zero16();
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lv, 32 * t, i, lane), gf[i], da);
-      f32x16 both;
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
         f32x16 s = zero16();
@@ -161,8 +151,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= (a == 0 ? da[r] : -lam * da[r]) - delta[a];
-        if (a == 0) both = s;
-        else both += s;
+        if (p.part && !side) {      // rows = this wave's queries, columns = keys; a lane adds its own second map's scores
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float* at = scr + (lane & 31) * SCR + acc_row(r, half);
+            *at = a == 0 ? s[r] : *at + s[r];
+          }
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           Frag<T> sf;
@@ -173,9 +168,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
       }
       if (p.part && !side) {
-        // rows = this wave's queries, columns = keys; then lane l sums diagonal key - query = l - 31 (63 of them)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) scr[(lane & 31) * SCR + acc_row(r, half)] = both[r];
+        // lane l sums diagonal key - query = l - 31 (63 of them)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         const int off = lane - 31;
@@ -259,9 +252,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *lq = lds, *lg = lds + TK::BYTES;
-  float* rows = (float*)(lds + 2 * TK::BYTES);                    // [MAPS][2][TILE]: -lse, delta
-  float* tab = rows + MAPS * 2 * TILE;
+  float* rows2 = (float*)(lds + Stream<T, D>::BYTES);             // two of [MAPS][2][TILE]: -lse, delta
+  float* tab = rows2 + 2 * MAPS * 2 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * 128, b = j0 / p.Hkv, hk = j0 % p.Hkv;
@@ -270,12 +262,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   const bool live = krow < limit;
   const T* kp = (const T*)p.k + b * p.kb + hk * p.kh + (long long)krow * p.ks;
   const T* vp = (const T*)p.v + b * p.vb + hk * p.vh + (long long)krow * p.vs;
-  Frag<T> kf[D / 16], vf[D / 16];
+  // fp32 at 128 columns: keys, values and both accumulators do not fit in 512 registers; the values come from the cache again for
+  // every tile (16 KiB against 8192 cycles of matrix instructions)
+  constexpr bool HOLD = sizeof(T) * D <= 256;
+  Frag<T> kf[D / 16], vf[HOLD ? D / 16 : 1];
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     kf[i] = frag_global(kp, i, lane, live);
-    vf[i] = frag_global(vp, i, lane, live);
+    if constexpr (HOLD) vf[i] = frag_global(vp, i, lane, live);
   }
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
@@ -284,15 +279,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   }
   const float c = p.scale * LOG2E;
   int first = 0;                                                  // first query row that sees a key of this block
-  if (p.causal) first = max(0, kblock - start) / TILE * TILE;
-  const int per = kblock < limit && first < p.Sq ? (p.Sq - first + TILE - 1) / TILE : 0, total = per * G;
-  u32x4 rq[TK::PER], rg[TK::PER];
+  if (p.causal) first = max(0, kblock - start) / TK::ROWS * TK::ROWS;
+  const int per = kblock < limit && first < p.Sq ? (p.Sq - first + TK::ROWS - 1) / TK::ROWS : 0, total = per * G;
+  Stream<T, D> qg(lds);
   float rl[MAPS], rd[MAPS];
   const auto fetch = [&](int it) {
-    const int h = hk * G + it / per, q0 = first + it % per * TILE;
-    TK::fetch(rq, (const T*)p.q + b * p.qb + h * p.qh, p.qs, q0, p.Sq, tid);
-    TK::fetch(rg, (const T*)p.d_o + ((size_t)b * p.Sq * p.H + h) * D, (long long)p.H * D, q0, p.Sq, tid);
-    if (tid < TILE)
+    const int h = hk * G + it / per, q0 = first + it % per * TK::ROWS;
+    qg.next((const T*)p.q + b * p.qb + h * p.qh, p.qs, (const T*)p.d_o + ((size_t)b * p.Sq * p.H + h) * D, (long long)p.H * D, q0, p.Sq, tid);
+    if (tid < TK::ROWS)
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
         const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + q0 + tid;
@@ -303,24 +297,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   if (total > 0) fetch(0);
   float lam = 0.f;
   for (int it = 0; it < total; ++it) {
-    const int h = hk * G + it / per, q0 = first + it % per * TILE;
-    __syncthreads();
-    TK::put(lq, rq, tid);
-    TK::put(lg, rg, tid);
-    if (tid < TILE)
+    const int h = hk * G + it / per, q0 = first + it % per * TK::ROWS;
+    float* rows = rows2 + (it & 1) * MAPS * 2 * TILE;            // written while other waves may still read the other one
+    if (tid < TK::ROWS)
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
         rows[a * 2 * TILE + tid] = -rl[a];
         rows[a * 2 * TILE + TILE + tid] = rd[a];
       }
-    if (it % per == 0) {
-      if (p.bk.n) fill_bias(p, tab, h, tid, 256);
+    qg.arrive();
+    char *lq = qg.a(), *lg = qg.b();
+    if (it % per == 0) {                                           // a head begins
       if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+      if (p.bk.n) {
+        fill_bias(p, tab, h, tid, 256);
+        __syncthreads();
+      }
     }
-    __syncthreads();
     if (it + 1 < total) fetch(it + 1);
 #pragma unroll 1
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TK::ROWS / 32; ++t) {
       const int r0 = q0 + 32 * t, qlo = start + r0, qhi = qlo + 31;
       if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
       const bool whole = khi < limit && (!p.causal || khi <= qlo);
@@ -334,7 +330,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       }
       f32x16 da = zero16(), mix;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lg, 32 * t, i, lane), vf[i], da);
+      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lg, 32 * t, i, lane), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da);
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
         f32x16 s = zero16();
@@ -435,11 +431,11 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
   p.delta = (float*)d->ws;
   if (d->dbias) p.part = p.delta + s.delta;
   if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
-  const size_t tiles = 2 * (size_t)Tile<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
+  const size_t tiles = (size_t)Stream<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
   const size_t sums = d->dbias ? 4 * (4 * (size_t)(2 * p.bk.reach + 1) + 4 * 32 * SCR) : 0;
   int rc = launch(attn_dq_kernel<T, D, MAPS>, (size_t)((p.Sq + 127) / 128) * p.B * p.H, 256, tiles + tab + sums, p, st, who);
   if (rc) return rc;
-  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 4 * MAPS * 2 * TILE, p, st, who);
+  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 2 * 4 * MAPS * 2 * TILE, p, st, who);
   if (rc) return rc;
   const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);
   if (outs == 0) return EOVAE_OK;

@@ -25,7 +25,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int MAX_BUCKETS = 128;       // per side: at most 64 borders behind the exact half
 constexpr int MAX_REACH = 1024;
-constexpr int TILE = 64;               // rows of a staged tile
+constexpr int TILE = 64;               // rows of a staged tile (Tile::ROWS), at most
 constexpr int PAD = 32 + TILE;         // a 32 x TILE tile that touches |rel| < reach stays inside [-reach - PAD, reach + PAD]
 
 // Buckets of one side: n < exact -> n, else exact + #{borders <= n}.  reach: first distance of the last bucket (everything
@@ -75,34 +75,57 @@ __device__ __forceinline__ float ldf(const void* p, size_t i, int is_f32) {
   return is_f32 ? ((const float*)p)[i] : (float)((const __bf16*)p)[i];
 }
 
-// ---- staged tiles: TILE rows of D elements, 16-byte chunks, chunk index XORed with swz(row) ----
+// 16 bytes per lane from `src` to LDS at `to` + 16 * lane.  The compiler does not count it: wait_dma() does.
+__device__ __forceinline__ void load_lds16(const void* src, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src) : "memory", "m0");
+}
+// until at most N of the wave's newest loads are still on their way
+template <int N> __device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// the wave's LDS reads are done: what they read may be overwritten
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// ---- staged tiles: ROWS rows of D elements, 16-byte chunks, chunk index XORed with swz(row) ----
 // Eight consecutive rows at one chunk index (a fragment read: lanes = rows) fall into eight different 16-byte bank groups,
 // and four consecutive rows times two consecutive chunks (a transposed 16-bit read) cover all 128 bytes once.
 template <typename T, int D> struct Tile {
+  static constexpr int ROWS = sizeof(T) * D > 256 ? 32 : TILE;   // fp32 rows of 128: half, so that two pairs of tiles and the sums fit in LDS
   static constexpr int ROWB = D * (int)sizeof(T);
   static constexpr int CH = ROWB / 16;                       // chunks per row: 4 .. 32
-  static constexpr int BYTES = TILE * ROWB;
-  static constexpr int PER = TILE * CH / 256;                // chunks per thread of a 256-thread block (1 .. 8)
+  static constexpr int BYTES = ROWS * ROWB;
+  static constexpr int PER = ROWS * CH / 256;                // chunks per thread of a 256-thread block (1 .. 4)
   static __device__ __forceinline__ int swz(int row) {
     return CH >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : ((row & 2) | ((row >> 2) & 1));
   }
   static __device__ __forceinline__ int at(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
 
-  // rows row0 .. row0 + TILE - 1 of a strided matrix; rows >= limit read as zero (never touched in memory)
-  static __device__ __forceinline__ void fetch(u32x4 (&r)[PER], const T* base, long long stride, int row0, int limit, int tid) {
+  // Rows row0 .. row0 + ROWS - 1 of a strided matrix straight into LDS (global_load_lds: a wave's 64 chunks of 16 bytes land one
+  // behind the other from the address in M0, so the swizzle is in what a lane ASKS for; 256 / CH rows further down it is the
+  // same).  Rows at and behind `limit` (>= 1) become copies of row limit - 1: finite wherever the caller's data is, and never
+  // visible.  A block of 256 threads calls; wait_dma<0>() before the barrier that publishes it.
+  static __device__ __forceinline__ void dma(const T* base, long long stride, int row0, int limit, const char* lds, int tid) {
+    const int row = tid / CH, col = ((tid % CH) ^ swz(row)) << 4;
+    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds +
+                                                                       (unsigned)(tid & ~63) * 16u));
+    if (row0 + ROWS <= limit) {
+      const char* src = (const char*)(base + (long long)row0 * stride + (long long)row * stride) + col;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = tid + 256 * i, row = c / CH, ch = c % CH;
-      u32x4 z = {0, 0, 0, 0};
-      if (row0 + row < limit) z = *(const u32x4*)((const char*)(base + (long long)(row0 + row) * stride) + ch * 16);
-      r[i] = z;
+      for (int i = 0; i < PER; ++i) load_lds16(src + (long long)i * (256 / CH) * stride * (long long)sizeof(T), to + 4096u * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = row0 + row + i * (256 / CH);
+        load_lds16((const char*)(base + (long long)(r < limit ? r : limit - 1) * stride) + col, to + 4096u * i);
+      }
     }
   }
-  static __device__ __forceinline__ void put(char* lds, const u32x4 (&r)[PER], int tid) {
+  // 32 rows by one wave for itself alone (32 CH / 64 loads): no barrier, only wait_dma
+  static constexpr int PER32 = 32 * CH / 64;
+  static __device__ __forceinline__ void dma32(const T* base, long long stride, int row0, int limit, const char* lds, int lane) {
+    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = tid + 256 * i;
-      *(u32x4*)(lds + at(c / CH, c % CH)) = r[i];
+    for (int i = 0; i < PER32; ++i) {
+      const int c = lane + 64 * i, row = c / CH, r = row0 + row;
+      load_lds16((const char*)(base + (long long)(r < limit ? r : limit - 1) * stride) + (((c % CH) ^ swz(row)) << 4), to + 1024u * i);
     }
   }
   // operand fragment: lane holds row (row0 + l % 32), columns 16 s + 8 (l / 32) .. + 7
@@ -139,6 +162,30 @@ template <typename T, int D> struct Tile {
       }
     }
     return f;
+  }
+};
+
+// Two row streams (keys and values, or queries and upstream gradients) through LDS, one tile of each at a time: two buffers,
+// the next pair arrives by DMA while this one is used, one barrier per tile.
+//   next(...)      request a pair of tiles
+//   arrive()       they are in LDS for every wave: a(), b() until the next arrive; the pair before is free
+template <typename T, int D> struct Stream {
+  using TK = Tile<T, D>;
+  static constexpr int BYTES = 4 * TK::BYTES;
+  char* lds;
+  int flip;
+  __device__ __forceinline__ explicit Stream(char* l) : lds(l), flip(0) {}
+  __device__ __forceinline__ char* a() const { return lds + flip * 2 * TK::BYTES; }
+  __device__ __forceinline__ char* b() const { return a() + TK::BYTES; }
+  __device__ __forceinline__ void next(const T* pa, long long sa, const T* pb, long long sb, int row0, int limit, int tid) {
+    char* to = lds + (flip ^ 1) * 2 * TK::BYTES;
+    TK::dma(pa, sa, row0, limit, to, tid);
+    TK::dma(pb, sb, row0, limit, to + TK::BYTES, tid);
+  }
+  __device__ __forceinline__ void arrive() {
+    wait_dma<0>();
+    __syncthreads();
+    flip ^= 1;
   }
 };
 

@@ -14,6 +14,8 @@ using namespace tok;
 
 namespace {
 
+constexpr int STEP_BLOCKS = 1024;      // blocks that a step-form call is split into
+
 // Scores of one wave's 32 queries against 32 NT keys, turned into probabilities in place (relative to 2^m, not normalised);
 // returns the factor by which the wave's earlier sums have to be multiplied (`moved`: whether any lane's differs from 1).
 // The reference m of a row is its maximum when it last moved: it follows only when a score passes it by 2^SLACK, which the
@@ -123,12 +125,10 @@ template <typename T, int N> __device__ __forceinline__ float positive_scale(flo
 
 template <typename T, int D, int MAPS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const Params p) {
-  using TK = Tile<T, D>;
   constexpr int W = D / MAPS;                 // width of one map's queries and keys
   constexpr int RB = 128 / MAPS;              // query rows of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *lk = lds, *lv = lds + TK::BYTES;
-  float* tab = (float*)(lds + 2 * TK::BYTES);
+  float* tab = (float*)(lds + Stream<T, D>::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int map = MAPS == 2 ? wave >> 1 : 0, wrow = 32 * (MAPS == 2 ? (wave & 1) : wave);
   const int nbh = p.B * p.H, tiles = (p.Sq + RB - 1) / RB;
@@ -154,22 +154,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   float m = -INFINITY, l = 0.f;
-  u32x4 rk[TK::PER], rv[TK::PER];
-  if (kend > 0) {
-    TK::fetch(rk, kb, p.ks, 0, limit, tid);
-    TK::fetch(rv, vb, p.vs, 0, limit, tid);
-  }
-  for (int k0 = 0; k0 < kend; k0 += TILE) {
-    __syncthreads();
-    TK::put(lk, rk, tid);
-    TK::put(lv, rv, tid);
-    __syncthreads();
-    if (k0 + TILE < kend) {
-      TK::fetch(rk, kb, p.ks, k0 + TILE, limit, tid);
-      TK::fetch(rv, vb, p.vs, k0 + TILE, limit, tid);
-    }
+  Stream<T, D> kv(lds);
+  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
+  constexpr int ROWS = Tile<T, D>::ROWS;
+  for (int k0 = 0; k0 < kend; k0 += ROWS) {
+    kv.arrive();
+    if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, limit, tid);
     if (!p.causal || k0 <= qhi)
-      tile_step<T, D, W, 2>(p, lk, lv, qf, acc, m, l, c, map, k0, limit, qpos, qlo, qhi, tab, lane);
+      tile_step<T, D, W, ROWS / 32>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, k0, limit, qpos, qlo, qhi, tab, lane);
   }
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -220,13 +212,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
 // part (fp32): per (b, key head, row block, split, map): [32 rows][D] unnormalised sums, then per row (maximum, sum)
 template <int D, int MAPS> constexpr int part_floats() { return MAPS * 32 * (D + 2); }
 
+// A wave streams its own 32-key tiles (every WAVES-th of the block's chunk) through two private buffers: it waits for its own
+// loads only, so no barrier stands between the waves until they meet at the end, and one tile is on its way while one is used.
+template <typename T, int D> constexpr int step_waves() { return sizeof(T) * D > 256 ? 2 : 4; }
+
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
+__global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(const Params p) {
   using TK = Tile<T, D>;
-  constexpr int W = D / MAPS;
+  constexpr int W = D / MAPS, WAVES = step_waves<T, D>(), T32 = 32 * TK::ROWB;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *lk = lds, *lv = lds + 2 * TK::BYTES;                  // 128 keys: two tiles of K, two of V
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  char* mine = lds + wave * 4 * T32;                           // two of (K, V)
   const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
   int j = (int)blockIdx.x;
   const int split = j % p.splits;
@@ -244,13 +240,23 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
   const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
   const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qi * p.qs;
-  // bias: bucket per distance (one byte) and the key head's rows of the table; two LDS reads per score near the query
-  unsigned char* ids = (unsigned char*)(lds + 4 * TK::BYTES);
+  int k0 = k_lo + 32 * wave;
+  if (k0 < k_hi) {
+    TK::dma32(kb, p.ks, k0, k_hi, mine, lane);
+    TK::dma32(vb, p.vs, k0, k_hi, mine + T32, lane);
+  }
+  // bias: bucket per distance (one byte) and the key head's columns of the table; two LDS reads per score near the query, the
+  // last buckets' values (one pair per query head, so per lane) everywhere else
+  unsigned char* ids = (unsigned char*)(lds + WAVES * 4 * T32);
   const int reach = p.bk.reach;
   float* tab = (float*)(ids + (p.bk.n ? ((2 * reach + 1 + 15) & ~15) : 0));
+  float far_l = 0.f, far_r = 0.f;
   if (p.bk.n) {
-    for (int i = tid; i <= 2 * reach; i += 256) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
-    for (int i = tid; i < p.bk.n * G; i += 256) tab[i] = ldf(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32) * LOG2E;
+    for (int i = tid; i <= 2 * reach; i += 64 * WAVES) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
+    for (int i = tid; i < p.bk.n * G; i += 64 * WAVES) tab[i] = ldf(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32) * LOG2E;
+    __syncthreads();
+    far_l = tab[ids[0] * G + g];
+    far_r = tab[ids[2 * reach] * G + g];
   }
   Frag<T> qf[D / 16];
 #pragma unroll
@@ -265,52 +271,39 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
     for (int i = 0; i < D / 32; ++i) acc[a][i] = zero16();
   }
   const float c = positive_scale(p.scale, qf);
-  u32x4 rk[2][TK::PER], rv[2][TK::PER];
-  if (k_lo < k_hi)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      TK::fetch(rk[t], kb, p.ks, k_lo + TILE * t, k_hi, tid);
-      TK::fetch(rv[t], vb, p.vs, k_lo + TILE * t, k_hi, tid);
+  for (int flip = 0; k0 < k_hi; k0 += 32 * WAVES, flip ^= 1) {
+    char *wk = mine + flip * 2 * T32, *wv = wk + T32;
+    wait_reads();
+    if (k0 + 32 * WAVES < k_hi) {
+      char* to = mine + (flip ^ 1) * 2 * T32;
+      TK::dma32(kb, p.ks, k0 + 32 * WAVES, k_hi, to, lane);
+      TK::dma32(vb, p.vs, k0 + 32 * WAVES, k_hi, to + T32, lane);
+      wait_dma<2 * TK::PER32>();
+    } else {
+      wait_dma<0>();
     }
-  for (int k0 = k_lo; k0 < k_hi; k0 += 2 * TILE) {
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      TK::put(lk + t * TK::BYTES, rk[t], tid);
-      TK::put(lv + t * TK::BYTES, rv[t], tid);
-    }
-    __syncthreads();
-    if (k0 + 2 * TILE < k_hi)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        TK::fetch(rk[t], kb, p.ks, k0 + 2 * TILE + TILE * t, k_hi, tid);
-        TK::fetch(rv[t], vb, p.vs, k0 + 2 * TILE + TILE * t, k_hi, tid);
-      }
-    const int kw = k0 + 32 * wave;                                // this wave's 32 keys
-    if (kw >= k_hi) continue;
-    char *wk = lk + (wave >> 1) * TK::BYTES, *wv = lv + (wave >> 1) * TK::BYTES;
-    const int r0 = 32 * (wave & 1);
+    const bool near = p.bk.n && k0 + 31 - start > -reach && k0 - (start + p.Sq - 1) < reach;
+    const float far = k0 + 31 - start <= -reach ? far_l : far_r;
+    const int last = min(k_hi - 1, p.causal ? qpos : 0x7fffffff) - k0 - 4 * half;                // last visible key of this lane's query
 #pragma unroll
     for (int a = 0; a < MAPS; ++a) {
       f32x16 s = zero16();
 #pragma unroll
-      for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(wk, r0, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
+      for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(wk, 0, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
       float top = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int k = kw + acc_row(r, half);
-        float x = s[r] * c;
-        if (p.bk.n) {
-          int rel = k - qpos;
+        const int k = 8 * (r >> 2) + (r & 3);
+        float add = far;
+        if (near) {
+          int rel = k0 + 4 * half + k - qpos;
           rel = rel < -reach ? -reach : (rel > reach ? reach : rel);
-          x += tab[ids[rel + reach] * G + g];
+          add = tab[ids[rel + reach] * G + g];
         }
-        if (k >= k_hi || (p.causal && k > qpos)) x = -INFINITY;
-        s[r] = x;
-        top = fmaxf(top, x);
+        s[r] = k > last ? -INFINITY : fmaf(s[r], c, add);
+        top = fmaxf(top, s[r]);
       }
-      top = column_max(top);
-      const float mn = fmaxf(m[a], top), base = mn == -INFINITY ? 0.f : mn, al = exp2_(m[a] - base);
+      const float mn = fmaxf(m[a], column_max(top)), base = mn == -INFINITY ? 0.f : mn, al = exp2_(m[a] - base);
       m[a] = mn;
       float sum = 0.f;
 #pragma unroll
@@ -326,14 +319,14 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
         Frag<T> pf;
         to_frag(pf, s, 8 * u);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[a][i] = mma(TK::frag_t(wv, r0 + 16 * u, 32 * i, lane), pf, acc[a][i]);
+        for (int i = 0; i < D / 32; ++i) acc[a][i] = mma(TK::frag_t(wv, 16 * u, 32 * i, lane), pf, acc[a][i]);
       }
     }
   }
-  // join the four waves: [wave][32 rows][D + 4] sums and [wave][32][2] statistics, one map at a time
+  // join the waves: [wave][32 rows][D + 4] sums and [wave][32][2] statistics, one map at a time
   constexpr int MROW = D + 4;
   float* meet = (float*)lds;
-  float* stat = meet + 4 * 32 * MROW;
+  float* stat = meet + WAVES * 32 * MROW;
   float* out = p.part + (size_t)blockIdx.x * part_floats<D, MAPS>();
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
@@ -344,25 +337,26 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
       stat[(wave * 32 + col) * 2] = m[a];
       stat[(wave * 32 + col) * 2 + 1] = lt;
     }
+    if (live)
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 v = {acc[a][i][4 * q], acc[a][i][4 * q + 1], acc[a][i][4 * q + 2], acc[a][i][4 * q + 3]};
-        *(f32x4*)(meet + (wave * 32 + col) * MROW + 32 * i + 8 * q + 4 * half) = v;
-      }
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v = {acc[a][i][4 * q], acc[a][i][4 * q + 1], acc[a][i][4 * q + 2], acc[a][i][4 * q + 3]};
+          *(f32x4*)(meet + (wave * 32 + col) * MROW + 32 * i + 8 * q + 4 * half) = v;
+        }
     __syncthreads();
-    for (int i = tid; i < 32 * D / 4; i += 256) {
+    for (int i = tid; i < 32 * D / 4; i += 64 * WAVES) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      if (rb * 32 + r >= rows) continue;
+      if (rb * 32 + r >= rows) break;
       float mm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, stat[(w * 32 + r) * 2]);
+      for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, stat[(w * 32 + r) * 2]);
       const float base = mm == -INFINITY ? 0.f : mm;
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
       float ls = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = exp2_(stat[(w * 32 + r) * 2] - base);
         ls += f * stat[(w * 32 + r) * 2 + 1];
         sum += f * *(const f32x4*)(meet + (w * 32 + r) * MROW + d);
@@ -376,40 +370,52 @@ __global__ __launch_bounds__(256) void attn_step_kernel(const Params p) {
   }
 }
 
-// joins the splits of a row: one block per (b, key head, row), threads = columns
-template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(D < 64 ? 64 : D) void attn_join_kernel(const Params p) {
+// joins the splits of a row: one block per (b, key head, row); thread = (4 columns, every RUNS-th split), runs joined in order
+constexpr int MAX_SPLITS = 256;
+template <typename T, int D, int MAPS> __global__ __launch_bounds__(256) void attn_join_kernel(const Params p) {
+  constexpr int LANES = D / 4, RUNS = 256 / LANES, PF = part_floats<D, MAPS>();
+  __shared__ float wt[MAX_SPLITS], red[8];
+  __shared__ __attribute__((aligned(16))) float sums[RUNS][D];
   const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
   const int row = (int)blockIdx.x % rows, bk = (int)blockIdx.x / rows, hk = bk % p.Hkv, b = bk / p.Hkv;
-  const int d = threadIdx.x, g = row / p.Sq, qi = row % p.Sq, h = hk * G + g;
-  const float* part = p.part + ((size_t)bk * rblocks + row / 32) * p.splits * part_floats<D, MAPS>();
-  float o[MAPS];
+  const int tid = threadIdx.x, d = 4 * (tid % LANES), run = tid / LANES, g = row / p.Sq, qi = row % p.Sq, h = hk * G + g;
+  const float* part = p.part + ((size_t)bk * rblocks + row / 32) * p.splits * PF;
+  f32x4 o[MAPS];
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
     const float* st = part + MAPS * 32 * D + (a * 32 + row % 32) * 2;
-    float mm = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, st[(size_t)s * part_floats<D, MAPS>()]);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float sum = 0.f, l = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float f = exp2_(st[(size_t)s * part_floats<D, MAPS>()] - base);
-      l += f * st[(size_t)s * part_floats<D, MAPS>() + 1];
-      if (d < D) sum += f * part[(size_t)s * part_floats<D, MAPS>() + (a * 32 + row % 32) * D + d];
+    const bool has = tid < p.splits;
+    const float ms = has ? st[(size_t)tid * PF] : -INFINITY, ls = has ? st[(size_t)tid * PF + 1] : 0.f;
+    const float wm = wave_max(ms);
+    __syncthreads();
+    if ((tid & 63) == 0) red[tid >> 6] = wm;
+    __syncthreads();
+    const float mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = mm == -INFINITY ? 0.f : mm, f = exp2_(ms - base);
+    if (has) wt[tid] = f;
+    const float ws = wave_sum(f * ls);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ws;
+    __syncthreads();
+    const float l = (red[4] + red[5]) + (red[6] + red[7]);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = run; s < p.splits; s += RUNS) sum += wt[s] * *(const f32x4*)(part + (size_t)s * PF + (a * 32 + row % 32) * D + d);
+    *(f32x4*)(&sums[run][d]) = sum;
+    __syncthreads();
+    if (run == 0) {
+#pragma unroll
+      for (int r = 1; r < RUNS; ++r) sum += *(const f32x4*)(&sums[r][d]);
+      o[a] = sum * (l > 0.f ? 1.f / l : 0.f);
     }
-    o[a] = l > 0.f ? sum / l : 0.f;
-    if (p.lse && d == 0) p.lse[(((size_t)b * p.H + h) * MAPS + a) * p.Sq + qi] = l > 0.f ? mm + __builtin_amdgcn_logf(l) : INFINITY;
+    if (p.lse && tid == 0) p.lse[(((size_t)b * p.H + h) * MAPS + a) * p.Sq + qi] = l > 0.f ? mm + __builtin_amdgcn_logf(l) : INFINITY;
   }
-  if (d >= D) return;
+  if (run) return;
   const size_t at = (((size_t)b * p.Sq + qi) * p.H + h) * D + d;
   if constexpr (MAPS == 2) {
-    if (p.out2) ((T*)p.out2)[at] = (T)o[1];
-    ((T*)p.out)[at] = (T)(o[0] - ldf(p.lam, h, p.lam_f32) * o[1]);
-  } else {
-    ((T*)p.out)[at] = (T)o[0];
+    if (p.out2) store4((T*)p.out2 + at, o[1][0], o[1][1], o[1][2], o[1][3]);
+    const float lam = ldf(p.lam, h, p.lam_f32);
+    o[0] -= lam * o[1];
   }
+  store4((T*)p.out + at, o[0][0], o[0][1], o[0][2], o[0][3]);
 }
-
-constexpr int STEP_KEYS = 2 * TILE;      // keys of one round of a step-form block
 
 struct Plan {
   bool step;
@@ -419,18 +425,20 @@ struct Plan {
 
 template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   Plan r{};
+  constexpr int WAVES = step_waves<T, D>(), KEYS = 32 * WAVES;
   const long long G = p.H / p.Hkv, rows = G * p.Sq;
   const size_t bias = p.bk.n ? (size_t)((2 * p.bk.reach + 16) & ~15) + 4 * (size_t)p.bk.n * G : 0;
-  const size_t meet = (size_t)4 * 32 * (D + 4) * 4 + 4 * 32 * 2 * 4;
-  r.lds = 4 * (size_t)Tile<T, D>::BYTES + bias;
+  const size_t meet = (size_t)WAVES * 32 * (D + 4) * 4 + WAVES * 32 * 2 * 4;
+  r.lds = WAVES * 4 * 32 * (size_t)Tile<T, D>::ROWB + bias;
   if (r.lds < meet) r.lds = meet;
   r.step = rows <= 32 && r.lds <= 160 * 1024;
   r.rblocks = (int)((rows + 31) / 32);
   if (!r.step) return r;
-  const long long base = (long long)p.B * p.Hkv * r.rblocks, most = (p.Sk + STEP_KEYS - 1) / STEP_KEYS;
-  long long want = (1024 + base - 1) / base;
+  const long long base = (long long)p.B * p.Hkv * r.rblocks, most = (p.Sk + KEYS - 1) / KEYS;
+  long long want = (STEP_BLOCKS + base - 1) / base;
   if (want > most) want = most;
-  r.chunk = (int)(((p.Sk + want - 1) / want + STEP_KEYS - 1) / STEP_KEYS * STEP_KEYS);
+  if (want > MAX_SPLITS) want = MAX_SPLITS;
+  r.chunk = (int)(((p.Sk + want - 1) / want + KEYS - 1) / KEYS * KEYS);
   r.splits = (p.Sk + r.chunk - 1) / r.chunk;
   r.part_bytes = (size_t)base * r.splits * part_floats<D, MAPS>() * 4;
   return r;
@@ -447,12 +455,12 @@ template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t w
     p.splits = r.splits;
     p.chunk = r.chunk;
     const size_t base = (size_t)p.B * p.Hkv;
-    const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 256, r.lds, p, st, who);
+    const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 64 * step_waves<T, D>(), r.lds, p, st, who);
     if (rc) return rc;
-    return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, D < 64 ? 64 : D, 0, p, st, who);
+    return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, 256, 0, p, st, who);
   }
   constexpr int RB = 128 / MAPS;
-  size_t lds = 2 * (size_t)Tile<T, D>::BYTES + 4 * (size_t)bias_entries(p.bk);
+  size_t lds = (size_t)Stream<T, D>::BYTES + 4 * (size_t)bias_entries(p.bk);
   if (MAPS == 2 && lds < (size_t)64 * (D + 4) * 4) lds = (size_t)64 * (D + 4) * 4;
   return launch(attn_rows_kernel<T, D, MAPS>, (size_t)((p.Sq + RB - 1) / RB) * p.B * p.H, 256, lds, p, st, who);
 }
