@@ -283,14 +283,19 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
       wait_dma<0>();
     }
     const bool near = p.bk.n && k0 + 31 - start > -reach && k0 - (start + p.Sq - 1) < reach;
+    const bool whole = k0 + 31 < k_hi && (!p.causal || k0 + 31 <= start);
     const float far = k0 + 31 - start <= -reach ? far_l : far_r;
-    const int last = min(k_hi - 1, p.causal ? qpos : 0x7fffffff) - k0 - 4 * half;                // last visible key of this lane's query
+    f32x16 s[MAPS];
+    float cc = c, off = far, al[MAPS];
+    bool up = false;
 #pragma unroll
     for (int a = 0; a < MAPS; ++a) {
-      f32x16 s = zero16();
+      s[a] = zero16();
 #pragma unroll
-      for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(wk, 0, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
-      float top = -INFINITY;
+      for (int i = 0; i < W / 16; ++i) s[a] = mma(TK::frag(wk, 0, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s[a]);
+    }
+    if (near || !whole) {
+      const int last = min(k_hi - 1, p.causal ? qpos : 0x7fffffff) - k0 - 4 * half;              // last visible key of this lane's query
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int k = 8 * (r >> 2) + (r & 3);
@@ -300,26 +305,52 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
           rel = rel < -reach ? -reach : (rel > reach ? reach : rel);
           add = tab[ids[rel + reach] * G + g];
         }
-        s[r] = k > last ? -INFINITY : fmaf(s[r], c, add);
-        top = fmaxf(top, s[r]);
+#pragma unroll
+        for (int a = 0; a < MAPS; ++a) s[a][r] = k > last ? -INFINITY : fmaf(s[a][r], c, add);
       }
-      const float mn = fmaxf(m[a], column_max(top)), base = mn == -INFINITY ? 0.f : mn, al = exp2_(m[a] - base);
-      m[a] = mn;
+      cc = 1.f;
+      off = 0.f;
+    }
+    // as in softmax_tile: the reference follows the maximum in steps of 2^SLACK
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      float top = s[a][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[a][r]);
+      al[a] = fmaf(column_max(top), cc, off);
+      up = up || al[a] > m[a] + SLACK;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        const float mn = fmaxf(m[a], al[a]), f = exp2_(m[a] - (mn == -INFINITY ? 0.f : mn));
+        m[a] = mn;
+        l[a] *= f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[a][i] *= f;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      const float base = off - (m[a] == -INFINITY ? 0.f : m[a]);
       float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = exp2_(s[r] - base);
-        sum += s[r];
+        s[a][r] = exp2_(fmaf(s[a][r], cc, base));
+        sum += s[a][r];
       }
-      l[a] = l[a] * al + sum;
+      l[a] += sum;
+    }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[a][i] *= al;
+    for (int u = 0; u < 2; ++u) {
+      Frag<T> pf[MAPS];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Frag<T> pf;
-        to_frag(pf, s, 8 * u);
+      for (int a = 0; a < MAPS; ++a) to_frag(pf[a], s[a], 8 * u);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[a][i] = mma(TK::frag_t(wv, 16 * u, 32 * i, lane), pf, acc[a][i]);
+      for (int i = 0; i < D / 32; ++i) {
+        const Frag<T> vt = TK::frag_t(wv, 16 * u, 32 * i, lane);
+#pragma unroll
+        for (int a = 0; a < MAPS; ++a) acc[a][i] = mma(vt, pf[a], acc[a][i]);
       }
     }
   }

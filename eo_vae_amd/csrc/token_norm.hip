@@ -72,32 +72,62 @@ template <int WPR, int K> __device__ __forceinline__ void row_sum(float (&v)[K],
   }
 }
 
-template <typename T, int WPR, int NV> struct Cols {
-  static constexpr int N = NV * 8;
-  int l, C, vec;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// a lane's columns of a row: NV runs of eight, run i at (64 WPR i + lane) * 8
+template <typename T, int WPR, int NV, bool VEC> struct Cols {
+  static constexpr int N = NV * 8, RAW = NV * (int)sizeof(T) / 2;
+  int l, C;                                   // VEC: rows and parameters can be read 16 bytes at a time (whole runs inside the row)
   __device__ __forceinline__ int col(int i) const { return (i * 64 * WPR + l) * 8; }
-  __device__ __forceinline__ void load(float (&o)[N], const T* row) const {
+  __device__ __forceinline__ bool in(int i) const { return (VEC ? col(i / 8) : col(i / 8) + i % 8) < C; }
+  struct Raw { u32x4 r[RAW]; };               // the row's bytes as they lie, requested one row ahead of their use
+  __device__ __forceinline__ void request(Raw& o, const T* row) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(i);
-      if (vec) {
-        if (c < C) {
-          if constexpr (sizeof(T) == 2) {
-            const bf16x8v v = *(const bf16x8v*)(row + c);
+      if constexpr (VEC) {
+        const int at = c < C ? c : 0;           // behind the row: its head again, cleared by take()
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[8 * i + e] = (float)v[e];
-          } else {
-            const f32x4 a = *(const f32x4*)(row + c), b = *(const f32x4*)(row + c + 4);
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) o.r[i * (int)sizeof(T) / 2 + k] = *(const u32x4*)((const char*)(row + at) + 16 * k);
+      } else if constexpr (sizeof(T) == 2) {
+        bf16x8v v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[8 * i + e] = a[e], o[8 * i + 4 + e] = b[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[8 * i + e] = 0.f;
-        }
+        for (int e = 0; e < 8; ++e) v[e] = row[c + e < C ? c + e : 0];
+        o.r[i] = __builtin_bit_cast(u32x4, v);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[8 * i + e] = c + e < C ? (float)row[c + e] : 0.f;
+        for (int k = 0; k < 2; ++k) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = row[c + 4 * k + e < C ? c + 4 * k + e : 0];
+          o.r[2 * i + k] = __builtin_bit_cast(u32x4, v);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void take(float (&o)[N], const Raw& w) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const bf16x8v v = __builtin_bit_cast(bf16x8v, w.r[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[8 * i + e] = (float)v[e];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f32x4 v = __builtin_bit_cast(f32x4, w.r[2 * i + k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[8 * i + 4 * k + e] = v[e];
+        }
+      }
+      if constexpr (VEC) {
+        if (col(i) >= C)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[8 * i + e] = 0.f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!in(8 * i + e)) o[8 * i + e] = 0.f;
       }
     }
   }
@@ -105,7 +135,7 @@ template <typename T, int WPR, int NV> struct Cols {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(i);
-      if (vec) {
+      if constexpr (VEC) {
         if (c < C) {
           if constexpr (sizeof(T) == 2) {
             bf16x8v v;
@@ -124,43 +154,95 @@ template <typename T, int WPR, int NV> struct Cols {
       }
     }
   }
+  __device__ __forceinline__ void store_param(const float (&o)[N], void* p, size_t off, int f32) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(i);
+      if constexpr (VEC) {
+        if (c < C) {
+          if (f32) {
+            *(f32x4*)((float*)p + off + c) = f32x4{o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3]};
+            *(f32x4*)((float*)p + off + c + 4) = f32x4{o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]};
+          } else {
+            bf16x8v v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (__bf16)o[8 * i + e];
+            *(bf16x8v*)((__bf16*)p + off + c) = v;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < C) stp(p, off + c + e, f32, o[8 * i + e]);
+      }
+    }
+  }
   // a parameter row of either type; absent: `none` everywhere inside the row, 0 behind it
   __device__ __forceinline__ void param(float (&o)[N], const void* p, size_t off, int f32, float none) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(i);
+      if (!p) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = col(i) + e;
-        o[8 * i + e] = c < C ? (p ? ldp(p, off + c, f32) : none) : 0.f;
+        for (int e = 0; e < 8; ++e) o[8 * i + e] = c + e < C ? none : 0.f;
+      } else if constexpr (VEC) {
+        const size_t at = off + (c < C ? c : 0);
+        if (f32) {
+          const f32x4 x = *(const f32x4*)((const float*)p + at), y = *(const f32x4*)((const float*)p + at + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[8 * i + e] = x[e], o[8 * i + 4 + e] = y[e];
+        } else {
+          const bf16x8v v = *(const bf16x8v*)((const __bf16*)p + at);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[8 * i + e] = (float)v[e];
+        }
+        if (c >= C)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[8 * i + e] = 0.f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[8 * i + e] = c + e < C ? ldp(p, off + c + e, f32) : 0.f;
       }
+    }
   }
 };
 
-template <typename T, int WPR, int NV, bool LAYER>
+template <typename T, int WPR, int NV, bool LAYER, bool VEC>
 __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_fwd_kernel(const NormArgs a) {
   constexpr int N = NV * 8, WAVES = WPR == 8 ? 8 : 4, SLOTS = WAVES / WPR;
   __shared__ float red[2 * 2 * WAVES];
-  const int wave = threadIdx.x >> 6, slot = wave / WPR;
-  const Cols<T, WPR, NV> cs{(int)(threadIdx.x % (64 * WPR)), a.C, a.vec};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / WPR;
+  const Cols<T, WPR, NV, VEC> cs{(int)(threadIdx.x % (64 * WPR)), a.C};
   int parity = 0;
-  float w1[N], b1[N], w2[N], b2[N], g[N];
+  float w1[N], w2[N], g[N], b1[LAYER ? N : 1], b2[LAYER ? N : 1];
   cs.param(w1, a.w1, 0, a.p_f32, 1.f);
-  cs.param(b1, a.b1, 0, a.p_f32, 0.f);
   cs.param(w2, a.w2, 0, a.p_f32, 1.f);
-  cs.param(b2, a.b2, 0, a.p_f32, 0.f);
+  if constexpr (LAYER) {
+    cs.param(b1, a.b1, 0, a.p_f32, 0.f);
+    cs.param(b2, a.b2, 0, a.p_f32, 0.f);
+  }
   const float n = (float)a.C;       // divided by, not multiplied with 1 / n: the mean of equal values is that value
-  long long held = -1;
-  for (long long r0 = (long long)blockIdx.x * SLOTS; r0 < a.rows; r0 += (long long)gridDim.x * SLOTS) {
+  long long until = 0;                                          // rows below it use the gate row in g
+  typename Cols<T, WPR, NV, VEC>::Raw rh, rx;
+  const long long step = (long long)gridDim.x * SLOTS;
+  const auto row_of = [&](long long r0) { return r0 + slot < a.rows ? r0 + slot : a.rows - 1; };   // an idle slot repeats a row and stores nothing
+  const auto request = [&](long long r0) {
+    cs.request(rh, (const T*)a.h + row_of(r0) * a.C);
+    cs.request(rx, (const T*)a.x + row_of(r0) * a.C);
+  };
+  request((long long)blockIdx.x * SLOTS);
+  for (long long r0 = (long long)blockIdx.x * SLOTS; r0 < a.rows; r0 += step) {
     const bool on = r0 + slot < a.rows;
-    const long long row = on ? r0 + slot : a.rows - 1;       // an idle slot of the last round repeats a row and stores nothing
-    const long long gr = a.gates ? row / a.per_gate : 0;
-    if (gr != held) {
-      cs.param(g, a.gate, (size_t)gr * a.C, a.p_f32, 1.f);
-      held = gr;
-    }
+    const long long row = row_of(r0);
     float h[N], x[N];
-    cs.load(h, (const T*)a.h + row * a.C);
-    cs.load(x, (const T*)a.x + row * a.C);
+    cs.take(h, rh);
+    cs.take(x, rx);
+    if (r0 + step < a.rows) request(r0 + step);
+    if (row >= until) {
+      const long long gr = a.gates ? row / a.per_gate : 0;
+      cs.param(g, a.gate, (size_t)gr * a.C, a.p_f32, 1.f);
+      until = a.gates ? (gr + 1) * a.per_gate : a.rows;
+    }
     float m1 = 0.f, m2 = 0.f, s[1];
     if (LAYER) {
       s[0] = 0.f;
@@ -172,13 +254,13 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_fwd_kernel(const No
     s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      h[i] = (cs.col(i / 8) + i % 8 < a.C) ? h[i] - m1 : 0.f;
+      if constexpr (LAYER) h[i] = cs.in(i) ? h[i] - m1 : 0.f;
       s[0] += h[i] * h[i];
     }
     row_sum<WPR, 1>(s, red, parity, wave, WAVES);
     const float r1 = 1.f / sqrtf(s[0] / n + a.eps);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = a.alpha * x[i] + g[i] * (h[i] * r1 * w1[i] + b1[i]);
+    for (int i = 0; i < N; ++i) x[i] = a.alpha * x[i] + g[i] * (LAYER ? h[i] * r1 * w1[i] + b1[LAYER ? i : 0] : h[i] * r1 * w1[i]);
     if (on) cs.store(x, (T*)a.y + row * a.C);
     float r2 = 0.f;
     if (a.z) {
@@ -192,13 +274,13 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_fwd_kernel(const No
       s[0] = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        x[i] = (cs.col(i / 8) + i % 8 < a.C) ? x[i] - m2 : 0.f;
+        if constexpr (LAYER) x[i] = cs.in(i) ? x[i] - m2 : 0.f;
         s[0] += x[i] * x[i];
       }
       row_sum<WPR, 1>(s, red, parity, wave, WAVES);
       r2 = 1.f / sqrtf(s[0] / n + a.eps);
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = x[i] * r2 * w2[i] + b2[i];
+      for (int i = 0; i < N; ++i) x[i] = LAYER ? x[i] * r2 * w2[i] + b2[LAYER ? i : 0] : x[i] * r2 * w2[i];
       if (on) cs.store(x, (T*)a.z + row * a.C);
     }
     if (a.stats && on && threadIdx.x % (64 * WPR) == 0) *(f32x4*)(a.stats + 4 * row) = f32x4{m1, r1, m2, r2};
@@ -207,21 +289,45 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_fwd_kernel(const No
 
 // A block's unit of rows lies inside one gate row (segs units to each), or is group_units whole gate rows.
 // part: [units][parts][C], parts: dw1, dw2, then db1, db2 (layer norms), then the gate row's dg when segs > 1
-template <typename T, int WPR, int NV, bool LAYER>
+// The next row's bytes are requested before this row is worked on (AHEAD), except where the registers do not allow it.
+template <typename T, int WPR, int NV, bool LAYER, bool VEC>
 __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_bwd_kernel(const NormArgs a) {
-  constexpr int N = NV * 8, WAVES = WPR == 8 ? 8 : 4, SLOTS = WAVES / WPR, LANES = 64 * WPR;
+  constexpr int N = NV * 8, WAVES = WPR == 8 ? 8 : 4, SLOTS = WAVES / WPR, LANES = 64 * WPR, PARTS = LAYER ? 5 : 3;
+  constexpr bool AHEAD = WPR < 8;
   __shared__ float red[2 * 2 * WAVES];
   __shared__ __attribute__((aligned(16))) float fold[SLOTS > 1 ? (SLOTS - 1) * LANES * (N + 4) : 1];
-  const int wave = threadIdx.x >> 6, slot = wave / WPR;
-  const Cols<T, WPR, NV> cs{(int)(threadIdx.x % LANES), a.C, a.vec};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / WPR;
+  const Cols<T, WPR, NV, VEC> cs{(int)(threadIdx.x % LANES), a.C};
   int parity = 0;
-  float w1[N], w2[N], b1[N], g[N];
-  float sA[N], sB[N], sW1[N], sB1[N], sW2[N], sB2[N];
+  float w1[N], w2[N], b1[LAYER ? N : 1], g[N];
+  // layer norms of the widest rows: the sums (of this thread's own columns) live in LDS, 512 threads leave 256 registers each
+  constexpr bool SIDE = WPR == 8 && LAYER;
+  __shared__ float side[SIDE ? 4 : 1][SIDE ? N : 1][SIDE ? 512 : 1];
+  float sA[SIDE ? 1 : N], sW2[SIDE ? 1 : N], sB[LAYER && !SIDE ? N : 1], sB2[LAYER && !SIDE ? N : 1];
   cs.param(w1, a.w1, 0, a.p_f32, 1.f);
-  cs.param(b1, a.b1, 0, a.p_f32, 0.f);
+  if constexpr (LAYER) cs.param(b1, a.b1, 0, a.p_f32, 0.f);
   cs.param(w2, a.w2, 0, a.p_f32, 1.f);
+  const auto clear = [&](auto& v) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) sA[i] = sB[i] = sW1[i] = sB1[i] = sW2[i] = sB2[i] = 0.f;
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+  };
+  const auto clear_ab = [&]() {
+    if constexpr (SIDE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) side[0][i][threadIdx.x] = side[2][i][threadIdx.x] = 0.f;
+    } else {
+      clear(sA);
+      if constexpr (LAYER) clear(sB);
+    }
+  };
+  clear_ab();
+  if constexpr (SIDE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) side[1][i][threadIdx.x] = side[3][i][threadIdx.x] = 0.f;
+  } else {
+    clear(sW2);
+    if constexpr (LAYER) clear(sB2);
+  }
   const float n = (float)a.C;       // divided by, not multiplied with 1 / n: the mean of equal values is that value
   const long long gates = a.gates ? a.gates : 1;
   const bool single = a.per_gate == 1 && a.gates;              // a gate row per token: its gradient leaves with the token
@@ -240,6 +346,18 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_bwd_kernel(const No
     }
   };
   const long long unit = blockIdx.x;
+  float* part = a.part + (size_t)unit * PARTS * a.C;
+  // slot 0: v (times the gate row, for `gated`) into part `which`; `more`: onto what an earlier gate row of this unit left there
+  const auto keep = [&](const float (&v)[N], int which, bool gated, bool more) {
+    if (slot == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (cs.in(i)) {
+          float* at = part + (size_t)which * a.C + cs.col(i / 8) + i % 8;
+          const float x = gated ? g[i] * v[i] : v[i];
+          *at = more ? *at + x : x;
+        }
+  };
   long long g0, g1, ra, rb;                                    // gate rows [g0, g1), tokens [ra, rb) of each
   if (a.segs > 0) {
     g0 = unit / a.segs;
@@ -252,114 +370,123 @@ __global__ __launch_bounds__(WPR == 8 ? 512 : 256) void norm_bwd_kernel(const No
     ra = 0;
     rb = a.per_gate;
   }
-  const long long first = single ? g0 : 0, count = single ? g1 - g0 : 0;
+  typename Cols<T, WPR, NV, VEC>::Raw rh, rx, rd, rq;
+  f32x4 rs;
   for (long long gr = g0; gr < (single ? g0 + 1 : g1); ++gr) {
     if (!single) cs.param(g, a.gate, (size_t)gr * a.C, a.p_f32, 1.f);
-    const long long lo = single ? 0 : ra, hi = single ? count : rb, base = single ? first : gr * a.per_gate;
+    const long long lo = single ? 0 : ra, hi = single ? g1 - g0 : rb, base = single ? g0 : gr * a.per_gate;
+    const auto row_of = [&](long long r0) { return base + (r0 + slot < hi ? r0 + slot : hi - 1); };
+    const auto request = [&](long long r0) {
+      const long long at = row_of(r0) * a.C;
+      cs.request(rh, (const T*)a.h + at);
+      cs.request(rx, (const T*)a.x + at);
+      cs.request(rd, (const T*)a.dy + at);
+      if (a.dz) cs.request(rq, (const T*)a.dz + at);
+      rs = *(const f32x4*)(a.stats + 4 * row_of(r0));
+    };
+    if (AHEAD) request(lo);
     for (long long r0 = lo; r0 < hi; r0 += SLOTS) {
       const bool on = r0 + slot < hi;
-      const long long row = base + (on ? r0 + slot : hi - 1);
+      const long long row = row_of(r0);
+      if (!AHEAD) request(r0);
       if (single) cs.param(g, a.gate, (size_t)row * a.C, a.p_f32, 1.f);
       float h[N], y[N], d[N], q[N];
-      cs.load(h, (const T*)a.h + row * a.C);
-      cs.load(y, (const T*)a.x + row * a.C);
-      cs.load(d, (const T*)a.dy + row * a.C);
-      if (a.dz) cs.load(q, (const T*)a.dz + row * a.C);
-      const f32x4 st = *(const f32x4*)(a.stats + 4 * row);
-#pragma unroll
-      for (int i = 0; i < N; ++i) h[i] = (cs.col(i / 8) + i % 8 < a.C) ? (h[i] - st[0]) * st[1] : 0.f;
-      if (a.dz) {
-        float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float t = a.alpha * y[i] + g[i] * (h[i] * w1[i] + b1[i]);
-          y[i] = (cs.col(i / 8) + i % 8 < a.C) ? (t - st[2]) * st[3] : 0.f;
-          s[0] += q[i] * w2[i] * y[i];
-          s[1] += q[i] * w2[i];
-          if (on) {
-            sW2[i] += q[i] * y[i];
-            sB2[i] += q[i];
-          }
-        }
-        row_sum<WPR, 2>(s, red, parity, wave, WAVES);
-        const float ma = LAYER ? s[1] / n : 0.f, mt = s[0] / n;
-#pragma unroll
-        for (int i = 0; i < N; ++i) d[i] += st[3] * (q[i] * w2[i] - ma - y[i] * mt);
-      }
-      float s[2] = {0.f, 0.f};
+      cs.take(h, rh);
+      cs.take(y, rx);
+      cs.take(d, rd);
+      if (a.dz) cs.take(q, rq);
+      const f32x4 st = rs;
+      if (AHEAD && r0 + SLOTS < hi) request(r0 + SLOTS);
+      // columns behind the row are zero everywhere (a layer norm's mean has to be kept out of them)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (!(cs.col(i / 8) + i % 8 < a.C)) d[i] = 0.f;
-        const float c = d[i] * g[i] * w1[i];
+        h[i] = (h[i] - (LAYER ? st[0] : 0.f)) * st[1];
+        if (LAYER && !cs.in(i)) h[i] = 0.f;
+      }
+      if (a.dz) {
+        float s[LAYER ? 2 : 1] = {};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float t = a.alpha * y[i] + g[i] * (LAYER ? h[i] * w1[i] + b1[LAYER ? i : 0] : h[i] * w1[i]);
+          y[i] = (t - (LAYER ? st[2] : 0.f)) * st[3];
+          if (LAYER && !cs.in(i)) y[i] = 0.f;
+          const float e = q[i] * w2[i];
+          s[0] += e * y[i];
+          if constexpr (LAYER) s[1] += e;
+          if (on) {
+            if constexpr (SIDE) side[3][i][threadIdx.x] += q[i] * y[i];
+            else sW2[i] += q[i] * y[i];
+            if constexpr (SIDE) side[1][i][threadIdx.x] += q[i];
+            else if constexpr (LAYER) sB2[i] += q[i];
+          }
+          q[i] = e;
+        }
+        row_sum<WPR, LAYER ? 2 : 1>(s, red, parity, wave, WAVES);
+        const float mt = s[0] / n, ma = LAYER ? s[LAYER ? 1 : 0] / n : 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          d[i] += st[3] * (LAYER ? q[i] - ma - y[i] * mt : q[i] - y[i] * mt);
+          if (LAYER && !cs.in(i)) d[i] = 0.f;
+        }
+      }
+      float s[LAYER ? 2 : 1] = {};
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float e = d[i] * g[i], c = e * w1[i];
         s[0] += c * h[i];
-        s[1] += c;
+        if constexpr (LAYER) s[1] += c;
         y[i] = a.alpha * d[i];
+        q[i] = c;
         if (on) {
-          sA[i] += d[i] * h[i];
-          sB[i] += d[i];
+          if constexpr (SIDE) side[2][i][threadIdx.x] += (single ? e : d[i]) * h[i];
+          else sA[i] += (single ? e : d[i]) * h[i];
+          if constexpr (SIDE) side[0][i][threadIdx.x] += single ? e : d[i];
+          else if constexpr (LAYER) sB[i] += single ? e : d[i];
         }
       }
       if (on) cs.store(y, (T*)a.dx + row * a.C);
-      row_sum<WPR, 2>(s, red, parity, wave, WAVES);
-      const float mc = LAYER ? s[1] / n : 0.f, mu = s[0] / n;
+      row_sum<WPR, LAYER ? 2 : 1>(s, red, parity, wave, WAVES);
+      const float mu = s[0] / n, mc = LAYER ? s[LAYER ? 1 : 0] / n : 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = st[1] * (d[i] * g[i] * w1[i] - mc - h[i] * mu);
+      for (int i = 0; i < N; ++i) y[i] = st[1] * (LAYER ? q[i] - mc - h[i] * mu : q[i] - h[i] * mu);
       if (on) cs.store(y, (T*)a.dh + row * a.C);
-      if (single) {
+      if (single && on && a.dgate) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          sW1[i] += g[i] * sA[i];
-          sB1[i] += g[i] * sB[i];
-          y[i] = w1[i] * sA[i] + b1[i] * sB[i];
-          sA[i] = sB[i] = 0.f;
-        }
-        if (on && a.dgate)
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (cs.col(i / 8) + i % 8 < a.C) stp(a.dgate, (size_t)row * a.C + cs.col(i / 8) + i % 8, a.p_f32, y[i]);
+        for (int i = 0; i < N; ++i) y[i] = d[i] * (LAYER ? h[i] * w1[i] + b1[LAYER ? i : 0] : h[i] * w1[i]);
+        cs.store_param(y, a.dgate, (size_t)row * a.C, a.p_f32);
       }
+    }
+    float u[N], v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] = SIDE ? side[SIDE ? 2 : 0][SIDE ? i : 0][SIDE ? threadIdx.x : 0] : sA[SIDE ? 0 : i];
+    join(u);
+    keep(u, 0, !single, gr > g0);
+    if constexpr (LAYER) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = SIDE ? side[0][SIDE ? i : 0][SIDE ? threadIdx.x : 0] : sB[SIDE ? 0 : i];
+      join(v);
+      keep(v, 2, !single, gr > g0);
     }
     if (!single) {
-      join(sA);
-      if (LAYER) join(sB);
-      if (slot == 0) {
-        float* pd = a.part ? a.part + ((size_t)unit * (LAYER ? 5 : 3) + (LAYER ? 4 : 2)) * a.C : nullptr;
+      if (slot == 0 && a.dgate) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = cs.col(i / 8) + i % 8;
-          sW1[i] += g[i] * sA[i];
-          sB1[i] += g[i] * sB[i];
-          const float v = w1[i] * sA[i] + b1[i] * sB[i];
-          if (c < a.C && a.dgate) {
-            if (a.segs > 1) pd[c] = v;
-            else stp(a.dgate, (size_t)gr * a.C + c, a.p_f32, v);
-          }
-        }
+        for (int i = 0; i < N; ++i) v[i] = LAYER ? w1[i] * u[i] + b1[LAYER ? i : 0] * v[i] : w1[i] * u[i];
+        if (a.segs > 1) keep(v, PARTS - 1, false, false);
+        else cs.store_param(v, a.dgate, (size_t)gr * a.C, a.p_f32);
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) sA[i] = sB[i] = 0.f;
+      clear_ab();
     }
   }
-  if (single) {
-    join(sW1);
-    if (LAYER) join(sB1);
-  }
-  join(sW2);
-  if (LAYER) join(sB2);
-  if (slot == 0) {
-    float* pu = a.part + (size_t)unit * (LAYER ? 5 : 3) * a.C;
+  float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = cs.col(i / 8) + i % 8;
-      if (c < a.C) {
-        pu[c] = sW1[i];
-        pu[a.C + c] = sW2[i];
-        if (LAYER) {
-          pu[2 * a.C + c] = sB1[i];
-          pu[3 * a.C + c] = sB2[i];
-        }
-      }
-    }
+  for (int i = 0; i < N; ++i) v[i] = SIDE ? side[SIDE ? 3 : 0][SIDE ? i : 0][SIDE ? threadIdx.x : 0] : sW2[SIDE ? 0 : i];
+  join(v);
+  keep(v, 1, false, false);
+  if constexpr (LAYER) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = SIDE ? side[SIDE ? 1 : 0][SIDE ? i : 0][SIDE ? threadIdx.x : 0] : sB2[SIDE ? 0 : i];
+    join(v);
+    keep(v, 3, false, false);
   }
 }
 
@@ -381,6 +508,7 @@ __global__ __launch_bounds__(1024) void norm_fold_kernel(const NormArgs a, int u
   const int len = (n + 15) / 16, lo = run * len, hi = min(n, lo + len);
   float sum = 0.f;
   if (c < a.C)
+#pragma unroll 8
     for (int u = lo; u < hi; ++u) sum += a.part[((size_t)(u0 + u) * parts + which) * a.C + c];
   s[run][threadIdx.x & 63] = sum;
   __syncthreads();
@@ -454,7 +582,7 @@ NormArgs args_of(const eovae_token_norm* d) {
   a.rows = d->rows; a.C = d->channels; a.gates = (int)d->gates; a.layer = d->layer ? 1 : 0;
   a.p_f32 = d->param_dtype == EOVAE_F32;
   a.alpha = d->alpha; a.eps = d->eps;
-  const void* ptrs[] = {d->h, d->x, d->dy, d->dz, d->y, d->z, d->dh, d->dx};
+  const void* ptrs[] = {d->h, d->x, d->dy, d->dz, d->y, d->z, d->dh, d->dx, d->w1, d->b1, d->w2, d->b2, d->gate, d->dgate};
   bool vec = d->channels % 8 == 0;
   for (const void* p : ptrs) vec = vec && (size_t)p % 16 == 0;
   a.vec = vec;
@@ -462,20 +590,25 @@ NormArgs args_of(const eovae_token_norm* d) {
 }
 
 // waves per row and vectors per lane by the row's width
-#define NORM_WIDTHS(T, KERNEL, LAYER, blocks, st, a)                                                          \
-  do {                                                                                                         \
-    if ((a).C <= 512) hipLaunchKernelGGL((KERNEL<T, 1, 1, LAYER>), dim3(blocks), dim3(256), 0, st, a);          \
-    else if ((a).C <= 1024) hipLaunchKernelGGL((KERNEL<T, 1, 2, LAYER>), dim3(blocks), dim3(256), 0, st, a);    \
-    else if ((a).C <= 2048) hipLaunchKernelGGL((KERNEL<T, 2, 2, LAYER>), dim3(blocks), dim3(256), 0, st, a);    \
-    else if ((a).C <= 4096) hipLaunchKernelGGL((KERNEL<T, 4, 2, LAYER>), dim3(blocks), dim3(256), 0, st, a);    \
-    else hipLaunchKernelGGL((KERNEL<T, 8, 2, LAYER>), dim3(blocks), dim3(512), 0, st, a);                      \
+#define NORM_WIDTHS(T, KERNEL, LAYER, VEC, blocks, st, a)                                                          \
+  do {                                                                                                              \
+    if ((a).C <= 512) hipLaunchKernelGGL((KERNEL<T, 1, 1, LAYER, VEC>), dim3(blocks), dim3(256), 0, st, a);          \
+    else if ((a).C <= 1024) hipLaunchKernelGGL((KERNEL<T, 1, 2, LAYER, VEC>), dim3(blocks), dim3(256), 0, st, a);    \
+    else if ((a).C <= 2048) hipLaunchKernelGGL((KERNEL<T, 2, 2, LAYER, VEC>), dim3(blocks), dim3(256), 0, st, a);    \
+    else if ((a).C <= 4096) hipLaunchKernelGGL((KERNEL<T, 4, 2, LAYER, VEC>), dim3(blocks), dim3(256), 0, st, a);    \
+    else hipLaunchKernelGGL((KERNEL<T, 8, 2, LAYER, VEC>), dim3(blocks), dim3(512), 0, st, a);                      \
   } while (0)
-#define NORM_DISPATCH(KERNEL, f32, blocks, st, a)                          \
-  do {                                                                     \
-    if (f32 && (a).layer) NORM_WIDTHS(float, KERNEL, true, blocks, st, a);  \
-    else if (f32) NORM_WIDTHS(float, KERNEL, false, blocks, st, a);         \
-    else if ((a).layer) NORM_WIDTHS(__bf16, KERNEL, true, blocks, st, a);   \
-    else NORM_WIDTHS(__bf16, KERNEL, false, blocks, st, a);                 \
+#define NORM_TYPES(T, KERNEL, blocks, st, a)                                        \
+  do {                                                                              \
+    if ((a).layer && (a).vec) NORM_WIDTHS(T, KERNEL, true, true, blocks, st, a);     \
+    else if ((a).layer) NORM_WIDTHS(T, KERNEL, true, false, blocks, st, a);          \
+    else if ((a).vec) NORM_WIDTHS(T, KERNEL, false, true, blocks, st, a);            \
+    else NORM_WIDTHS(T, KERNEL, false, false, blocks, st, a);                        \
+  } while (0)
+#define NORM_DISPATCH(KERNEL, f32, blocks, st, a)              \
+  do {                                                         \
+    if (f32) NORM_TYPES(float, KERNEL, blocks, st, a);          \
+    else NORM_TYPES(__bf16, KERNEL, blocks, st, a);             \
   } while (0)
 
 }  // namespace
