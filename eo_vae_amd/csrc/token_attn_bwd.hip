@@ -23,18 +23,20 @@ using namespace tok;
 
 namespace {
 
-constexpr int SCR = 33;         // scratch row of a wave's 32 x 32 score-gradient tile (+ 1: diagonals spread over the banks)
+// a wave's score gradients by diagonal: 64 rows (63 distances) of 32 queries, 4 floats apart from the next row's banks
+constexpr int SCR = 36, SCR_FLOATS = 64 * SCR;
 
 template <typename T, int D, int MAPS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dq_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
+  constexpr int NT = D <= 64 && TK::ROWS == 64 ? 2 : 1;           // 32-key tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float* tab = (float*)(lds + Stream<T, D>::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach, ndiag = 2 * reach + 1;
-  float* diag = tab + ntab + wave * ndiag;                       // [4][2 reach + 1]: sums by distance, |distance| < reach used
-  float* scr = tab + ntab + 4 * ndiag + wave * 32 * SCR;
+  const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach;
+  float* diag = tab + ntab + wave * ntab;                        // [4][ntab]: sums of score gradients by distance
+  float* scr = tab + 5 * ntab + 3 - (5 * ntab + 3) % 4 + wave * SCR_FLOATS;
   const int nbh = p.B * p.H, tiles = (p.Sq + 127) / 128;
   const int tile = tiles - 1 - (int)blockIdx.x / nbh;
   int b, hk, h;
@@ -83,8 +85,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   }
   if (p.bk.n) {
     fill_bias(p, tab, h, tid, 256);
-    if (p.part)
-      for (int i = lane; i < ndiag; i += 64) diag[i] = 0.f;
+    if (p.part) {
+      for (int i = lane; i < ntab; i += 64) diag[i] = 0.f;
+      for (int i = lane; i < SCR_FLOATS; i += 64) scr[i] = 0.f;
+    }
   }
   f32x16 acc[D / 32];
 #pragma unroll
@@ -102,8 +106,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
     if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, limit, tid);
     char *lk = kv.a(), *lv = kv.b();
 #pragma unroll 1
-    for (int t = 0; t < TK::ROWS / 32; ++t) {
-      const int key0 = k0 + 32 * t, klast = key0 + 31;
+    for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT) {
+      const int key0 = k0 + 32 * t0, klast = key0 + 32 * NT - 1;
       if (key0 >= kend || (p.causal && key0 > qhi)) continue;
       const bool whole = klast < limit && (!p.causal || klast <= qlo);
       const float* tb = tab + (reach + PAD) + key0 - qpos + 4 * half;
@@ -115,75 +119,83 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
         else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
         else near = true;
       }
-      f32x16 da = zero16();
+      f32x16 da[NT];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lv, 32 * t, i, lane), gf[i], da);
+      for (int t = 0; t < NT; ++t) {
+        da[t] = zero16();
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) da[t] = mma(TK::frag(lv, 32 * (t0 + t), i, lane), gf[i], da[t]);
+      }
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
-        f32x16 s = zero16();
+        f32x16 s[NT];
 #pragma unroll
-        for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lk, 32 * t, a * (W / 16) + i, lane), qf[a * (W / 16) + i], s);
+        for (int t = 0; t < NT; ++t) {
+          s[t] = zero16();
+#pragma unroll
+          for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, 32 * (t0 + t), a * (W / 16) + i, lane), qf[a * (W / 16) + i], s[t]);
+        }
         float cc = c, off = far - lse[a];
         if (near || !whole) {
+          const int last = whole ? 0x7fffffff : min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, near ? tb[8 * (r >> 2) + (r & 3)] : far);
-          if (!whole) {
-            const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (8 * (r >> 2) + (r & 3) > last) s[r] = -INFINITY;
-          }
+            for (int r = 0; r < 16; ++r) {
+              const int k = 32 * t + 8 * (r >> 2) + (r & 3);
+              const float e = fmaf(s[t][r], c, near ? tb[k] : far);
+              s[t][r] = k > last ? -INFINITY : e;
+            }
           cc = 1.f;
           off = -lse[a];
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], cc, off));
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = exp2_(fmaf(s[t][r], cc, off));
         if (sums) {
           float xs = 0.f, ms = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            xs = fmaf(s[r], da[r], xs);
-            ms += s[r];
-          }
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              xs = fmaf(s[t][r], da[t][r], xs);
+              ms += s[t][r];
+            }
           x[a] += xs, m[a] += ms;
           if (side < 0) xl[a] += xs, ml[a] += ms;
           if (side > 0) xr[a] += xs, mr[a] += ms;
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= (a == 0 ? da[r] : -lam * da[r]) - delta[a];
-        if (p.part && !side) {      // rows = this wave's queries, columns = keys; a lane adds its own second map's scores
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float* at = scr + (lane & 31) * SCR + acc_row(r, half);
-            *at = a == 0 ? s[r] : *at + s[r];
+          for (int r = 0; r < 16; ++r) s[t][r] *= (a == 0 ? da[t][r] : -lam * da[t][r]) - delta[a];
+        if (p.part && !side) {
+          // [distance key - query + 31][query]: a lane writes its query's column, then lane l sums row l (63 of them); what lies
+          // outside the 32 x 32 tile stays zero from the start
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float* at = scr + (31 - (lane & 31) + 4 * half) * SCR + (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) at[(8 * (r >> 2) + (r & 3)) * SCR] = s[t][r];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) sum += *(const f32x4*)(scr + lane * SCR + 4 * q);
+            if (lane < 63) diag[(reach + PAD) + key0 + 32 * t - qlo + lane - 31] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          Frag<T> sf;
-          to_frag(sf, s, 8 * u);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < W / 32; ++j)
-            acc[a * (W / 32) + j] = mma(TK::frag_t(lk, 32 * t + 16 * u, a * W + 32 * j, lane), sf, acc[a * (W / 32) + j]);
-        }
-      }
-      if (p.part && !side) {
-        // lane l sums diagonal key - query = l - 31 (63 of them)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int off = lane - 31;
-        float sum = 0.f;
-        for (int q = 0; q < 32; ++q) {
-          const int k = q + off;
-          if (k >= 0 && k < 32) sum += scr[q * SCR + k];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int rel = key0 - qlo + off;
-        if (off > 31) sum = 0.f;                                   // lane 63: no diagonal
-        if (rel <= -reach) far_l += sum;
-        else if (rel >= reach) far_r += sum;
-        else if (off <= 31) diag[rel + reach] += sum;               // one lane per distance
+          for (int u = 0; u < 2; ++u) {
+            Frag<T> sf;
+            to_frag(sf, s[t], 8 * u);
+#pragma unroll
+            for (int j = 0; j < W / 32; ++j)
+              acc[a * (W / 32) + j] = mma(TK::frag_t(lk, 32 * (t0 + t) + 16 * u, a * W + 32 * j, lane), sf, acc[a * (W / 32) + j]);
+          }
       }
     }
   }
@@ -209,29 +221,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   const size_t slot = ((size_t)h * p.B + b) * tiles + tile;
   if (p.part) {
     __syncthreads();
-    float* fars = scr;
+    float* fars = (float*)lds;                                     // the tiles are done
     far_l = wave_sum(far_l);
     far_r = wave_sum(far_r);
     if (lane == 0) {
-      fars[0] = far_l;
-      fars[1] = far_r;
+      fars[2 * wave] = far_l;
+      fars[2 * wave + 1] = far_r;
+    }
+    // the four waves' sums into the first
+    float* d0 = tab + ntab;
+    for (int i = tid; i < ntab; i += 256) {
+      float sum = d0[i];
+      for (int w = 1; w < 4; ++w) sum += d0[w * ntab + i];
+      d0[i] = sum;
     }
     __syncthreads();
-    const float* d0 = tab + ntab;
-    const float* f0 = tab + ntab + 4 * ndiag;
+    const float* mid = d0 + reach + PAD;
     for (int u = tid; u < p.bk.n; u += 256) {
       const int right = p.bk.two_sided && u >= p.bk.side, i = right ? u - p.bk.side : u, last = p.bk.side - 1;
-      auto lo = [&](int x) { return x <= p.bk.exact ? x : p.bk.border[x - p.bk.exact - 1]; };
-      const int a = lo(i), z = i == last ? reach : lo(i + 1);         // distances a .. z - 1 (z = reach: the far sums hold the rest)
+      auto lo = [&](int n) { return n <= p.bk.exact ? n : p.bk.border[n - p.bk.exact - 1]; };
+      const int a = lo(i), z = i == last ? reach + PAD + 1 : lo(i + 1);    // distances a .. z - 1; behind them the far sums
       float sum = 0.f;
-      for (int w = 0; w < 4; ++w) {
-        for (int n = a; n < z; ++n) {
-          if (!right || n > 0) sum += d0[w * ndiag + reach + (right ? n : -n)];
-          if (!p.bk.two_sided && n == 0)
-            for (int e = 1; e < reach; ++e) sum += d0[w * ndiag + reach + e];     // one-sided: everything ahead is distance 0
-        }
-        if (i == last) sum += right ? f0[w * 32 * SCR + 1] : f0[w * 32 * SCR];
-        if (!p.bk.two_sided && i == 0) sum += f0[w * 32 * SCR + 1];
+      for (int n = a; n < z; ++n) sum += right ? (n > 0 ? mid[n] : 0.f) : mid[-n];
+      if (i == last)
+        for (int w = 0; w < 4; ++w) sum += fars[2 * w + right];
+      if (!p.bk.two_sided && i == 0) {                                     // one-sided: everything ahead is distance 0
+        for (int n = 1; n <= reach + PAD; ++n) sum += mid[n];
+        for (int w = 0; w < 4; ++w) sum += fars[2 * w + 1];
       }
       p.part[slot * p.bk.n + u] = sum;
     }
@@ -251,6 +267,7 @@ template <typename T, int D, int MAPS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_dkv_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
+  constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1;     // 32-query tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float* rows2 = (float*)(lds + Stream<T, D>::BYTES);             // two of [MAPS][2][TILE]: -lse, delta
   float* tab = rows2 + 2 * MAPS * 2 * TILE;
@@ -316,8 +333,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
     }
     if (it + 1 < total) fetch(it + 1);
 #pragma unroll 1
-    for (int t = 0; t < TK::ROWS / 32; ++t) {
-      const int r0 = q0 + 32 * t, qlo = start + r0, qhi = qlo + 31;
+    for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT) {
+      const int r0 = q0 + 32 * t0, qlo = start + r0, qhi = qlo + 32 * NT - 1;
       if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
       const bool whole = khi < limit && (!p.causal || khi <= qlo);
       const float* tb = tab + (reach + PAD) + krow - qlo - 4 * half;
@@ -328,55 +345,72 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
         else if (klo - qhi >= reach) far = tab[2 * (reach + PAD)];
         else near = true;
       }
-      f32x16 da = zero16(), mix;
+      f32x16 da[NT], mix[NT];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) da = mma(TK::frag(lg, 32 * t, i, lane), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da);
+      for (int t = 0; t < NT; ++t) {
+        da[t] = zero16();
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          da[t] = mma(TK::frag(lg, 32 * (t0 + t), i, lane), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da[t]);
+      }
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
-        f32x16 s = zero16();
+        f32x16 s[NT];
 #pragma unroll
-        for (int i = 0; i < W / 16; ++i) s = mma(TK::frag(lq, 32 * t, a * (W / 16) + i, lane), kf[a * (W / 16) + i], s);
-        const float* ls = rows + a * 2 * TILE + 32 * t;
+        for (int t = 0; t < NT; ++t) {
+          s[t] = zero16();
+#pragma unroll
+          for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lq, 32 * (t0 + t), a * (W / 16) + i, lane), kf[a * (W / 16) + i], s[t]);
+        }
+        const float* ls = rows + a * 2 * TILE + 32 * t0 + 4 * half;
         float cc = c;
         if (near || !whole || far != 0.f) {
+          // first query that sees this key
+          const int first = whole ? -0x7fffffff : (krow >= limit ? 0x7fffffff : (p.causal ? krow - qlo - 4 * half : -0x7fffffff));
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, near ? tb[-(8 * (r >> 2) + (r & 3))] : far);
-          if (!whole) {
-            const int first = krow >= limit ? 64 : (p.causal ? krow - qlo - 4 * half : 0);       // first query that sees this key
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (8 * (r >> 2) + (r & 3) < first) s[r] = -INFINITY;
-          }
+            for (int r = 0; r < 16; ++r) {
+              const int q = 32 * t + 8 * (r >> 2) + (r & 3);
+              const float e = fmaf(s[t][r], c, near ? tb[-q] : far);
+              s[t][r] = q < first ? -INFINITY : e;
+            }
           cc = 1.f;
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 nl = *(const f32x4*)(ls + 8 * g + 4 * half), dl = *(const f32x4*)(ls + TILE + 8 * g + 4 * half);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            const float x = exp2_(fmaf(s[r], cc, nl[e]));
-            if (a == 0) mix[r] = x;
-            else mix[r] = fmaf(-lam, x, mix[r]);
-            s[r] = x * ((a == 0 ? da[r] : -lam * da[r]) - dl[e]);
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 nl = *(const f32x4*)(ls + 32 * t + 8 * g), dl = *(const f32x4*)(ls + TILE + 32 * t + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * g + e;
+              const float x = exp2_(fmaf(s[t][r], cc, nl[e]));
+              if (a == 0) mix[t][r] = x;
+              else mix[t][r] = fmaf(-lam, x, mix[t][r]);
+              s[t][r] = x * ((a == 0 ? da[t][r] : -lam * da[t][r]) - dl[e]);
+            }
           }
-        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            Frag<T> sf;
+            to_frag(sf, s[t], 8 * u);
+#pragma unroll
+            for (int j = 0; j < W / 32; ++j)
+              dk[a * (W / 32) + j] = mma(TK::frag_t(lq, 32 * (t0 + t) + 16 * u, a * W + 32 * j, lane), sf, dk[a * (W / 32) + j]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          Frag<T> sf;
-          to_frag(sf, s, 8 * u);
+          Frag<T> pf;
+          to_frag(pf, mix[t], 8 * u);
 #pragma unroll
-          for (int j = 0; j < W / 32; ++j)
-            dk[a * (W / 32) + j] = mma(TK::frag_t(lq, 32 * t + 16 * u, a * W + 32 * j, lane), sf, dk[a * (W / 32) + j]);
+          for (int j = 0; j < D / 32; ++j) dv[j] = mma(TK::frag_t(lg, 32 * (t0 + t) + 16 * u, 32 * j, lane), pf, dv[j]);
         }
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Frag<T> pf;
-        to_frag(pf, mix, 8 * u);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) dv[j] = mma(TK::frag_t(lg, 32 * t + 16 * u, 32 * j, lane), pf, dv[j]);
-      }
     }
   }
   if (krow < p.Sk) {
@@ -432,7 +466,7 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
   if (d->dbias) p.part = p.delta + s.delta;
   if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
   const size_t tiles = (size_t)Stream<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
-  const size_t sums = d->dbias ? 4 * (4 * (size_t)(2 * p.bk.reach + 1) + 4 * 32 * SCR) : 0;
+  const size_t sums = d->dbias ? 4 * tab + 16 + 4 * 4 * SCR_FLOATS : 0;
   int rc = launch(attn_dq_kernel<T, D, MAPS>, (size_t)((p.Sq + 127) / 128) * p.B * p.H, 256, tiles + tab + sums, p, st, who);
   if (rc) return rc;
   rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 2 * 4 * MAPS * 2 * TILE, p, st, who);
