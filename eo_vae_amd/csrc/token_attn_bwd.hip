@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   f32x16 acc[D / 32];
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
-  const float c = p.scale * LOG2E;
+  const float c = positive_scale(p.scale, qf);
   // of this lane's query and map: sum P dA and sum P over the row, and over the keys of the two last buckets
   float x[MAPS], m[MAPS], xl[MAPS], xr[MAPS], ml[MAPS], mr[MAPS], far_l = 0.f, far_r = 0.f;
 #pragma unroll
@@ -137,15 +137,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
         }
         float cc = c, off = far - lse[a];
         if (near || !whole) {
-          const int last = whole ? 0x7fffffff : min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int k = 32 * t + 8 * (r >> 2) + (r & 3);
-              const float e = fmaf(s[t][r], c, near ? tb[k] : far);
-              s[t][r] = k > last ? -INFINITY : e;
-            }
+            for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, near ? tb[32 * t + 8 * (r >> 2) + (r & 3)] : far);
+          if (!whole) {
+            const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                if (32 * t + 8 * (r >> 2) + (r & 3) > last) s[t][r] = -INFINITY;
+          }
           cc = 1.f;
           off = -lse[a];
         }
@@ -269,8 +272,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   constexpr int W = D / MAPS;
   constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1;     // 32-query tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* rows2 = (float*)(lds + Stream<T, D>::BYTES);             // two of [MAPS][2][TILE]: -lse, delta
-  float* tab = rows2 + 2 * MAPS * 2 * TILE;
+  // two of [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it)
+  float* rows2 = (float*)(lds + Stream<T, D>::BYTES);
+  float* tab = rows2 + 2 * MAPS * 4 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * 128, b = j0 / p.Hkv, hk = j0 % p.Hkv;
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
     dk[j] = zero16();
     dv[j] = zero16();
   }
-  const float c = p.scale * LOG2E;
+  const float c = positive_scale(p.scale, kf);
   int first = 0;                                                  // first query row that sees a key of this block
   if (p.causal) first = max(0, kblock - start) / TK::ROWS * TK::ROWS;
   const int per = kblock < limit && first < p.Sq ? (p.Sq - first + TK::ROWS - 1) / TK::ROWS : 0, total = per * G;
@@ -312,25 +316,31 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       }
   };
   if (total > 0) fetch(0);
-  float lam = 0.f;
+  float lam = 0.f, far_l = 0.f, far_r = 0.f;
   for (int it = 0; it < total; ++it) {
     const int h = hk * G + it / per, q0 = first + it % per * TK::ROWS;
-    float* rows = rows2 + (it & 1) * MAPS * 2 * TILE;            // written while other waves may still read the other one
-    if (tid < TK::ROWS)
-#pragma unroll
-      for (int a = 0; a < MAPS; ++a) {
-        rows[a * 2 * TILE + tid] = -rl[a];
-        rows[a * 2 * TILE + TILE + tid] = rd[a];
-      }
-    qg.arrive();
-    char *lq = qg.a(), *lg = qg.b();
+    float* rows = rows2 + (it & 1) * MAPS * 4 * TILE;            // written while other waves may still read the other one
     if (it % per == 0) {                                           // a head begins
       if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
       if (p.bk.n) {
+        __syncthreads();
         fill_bias(p, tab, h, tid, 256);
         __syncthreads();
+        far_l = tab[PAD];
+        far_r = tab[2 * (reach + PAD)];
       }
     }
+    if (tid < TK::ROWS)
+#pragma unroll
+      for (int a = 0; a < MAPS; ++a) {
+        float* at = rows + a * 4 * TILE + tid;
+        at[0] = rd[a];
+        at[TILE] = -rl[a];
+        at[2 * TILE] = far_l - rl[a];
+        at[3 * TILE] = far_r - rl[a];
+      }
+    qg.arrive();
+    char *lq = qg.a(), *lg = qg.b();
     if (it + 1 < total) fetch(it + 1);
 #pragma unroll 1
     for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT) {
@@ -338,11 +348,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
       const bool whole = khi < limit && (!p.causal || khi <= qlo);
       const float* tb = tab + (reach + PAD) + krow - qlo - 4 * half;
-      float far = 0.f;
+      int offs = TILE;                                                 // which of a row's offsets
       bool near = false;
       if (p.bk.n) {
-        if (khi - qlo <= -reach) far = tab[PAD];
-        else if (klo - qhi >= reach) far = tab[2 * (reach + PAD)];
+        if (khi - qlo <= -reach) offs = 2 * TILE;
+        else if (klo - qhi >= reach) offs = 3 * TILE;
         else near = true;
       }
       f32x16 da[NT], mix[NT];
@@ -362,26 +372,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
 #pragma unroll
           for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lq, 32 * (t0 + t), a * (W / 16) + i, lane), kf[a * (W / 16) + i], s[t]);
         }
-        const float* ls = rows + a * 2 * TILE + 32 * t0 + 4 * half;
+        const float* ls = rows + a * 4 * TILE + 32 * t0 + 4 * half;
         float cc = c;
-        if (near || !whole || far != 0.f) {
-          // first query that sees this key
-          const int first = whole ? -0x7fffffff : (krow >= limit ? 0x7fffffff : (p.causal ? krow - qlo - 4 * half : -0x7fffffff));
+        if (near) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int q = 32 * t + 8 * (r >> 2) + (r & 3);
-              const float e = fmaf(s[t][r], c, near ? tb[-q] : far);
-              s[t][r] = q < first ? -INFINITY : e;
-            }
+            for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, tb[-(32 * t + 8 * (r >> 2) + (r & 3))]);
           cc = 1.f;
+        }
+        if (!whole) {       // first query that sees this key
+          const int first = krow >= limit ? 0x7fffffff : (p.causal ? krow - qlo - 4 * half : -0x7fffffff);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * t + 8 * (r >> 2) + (r & 3) < first) s[t][r] = -INFINITY;
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const f32x4 nl = *(const f32x4*)(ls + 32 * t + 8 * g), dl = *(const f32x4*)(ls + TILE + 32 * t + 8 * g);
+            const f32x4 nl = *(const f32x4*)(ls + offs + 32 * t + 8 * g), dl = *(const f32x4*)(ls + 32 * t + 8 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * g + e;
@@ -469,7 +481,7 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
   const size_t sums = d->dbias ? 4 * tab + 16 + 4 * 4 * SCR_FLOATS : 0;
   int rc = launch(attn_dq_kernel<T, D, MAPS>, (size_t)((p.Sq + 127) / 128) * p.B * p.H, 256, tiles + tab + sums, p, st, who);
   if (rc) return rc;
-  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 2 * 4 * MAPS * 2 * TILE, p, st, who);
+  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 2 * 4 * MAPS * 4 * TILE, p, st, who);
   if (rc) return rc;
   const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);
   if (outs == 0) return EOVAE_OK;

@@ -206,6 +206,17 @@ template <typename T> __device__ __forceinline__ Frag<T> frag_global(const T* ro
   return f;
 }
 
+// A negative scale is carried by one operand, and a scale of 0 becomes the smallest number: the largest product is the largest
+// score, and a masked -infinity stays one.  (In units of log 2.)
+template <typename T, int N> __device__ __forceinline__ float positive_scale(float scale, Frag<T> (&qf)[N]) {
+  if (scale < 0.f)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[i].x[e] = -qf[i].x[e];
+  return fmaxf(fabsf(scale) * LOG2E, 1.2e-38f);
+}
+
 // eight consecutive accumulator registers as the B operand of the next product
 __device__ __forceinline__ void to_frag(Frag<__bf16>& f, const f32x16& a, int r0) {
 #pragma unroll

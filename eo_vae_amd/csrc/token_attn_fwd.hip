@@ -113,16 +113,6 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
     }
 }
 
-// a negative scale is carried by the queries, so that the largest product is the largest score
-template <typename T, int N> __device__ __forceinline__ float positive_scale(float scale, Frag<T> (&qf)[N]) {
-  if (scale < 0.f)
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qf[i].x[e] = -qf[i].x[e];
-  return fabsf(scale) * LOG2E;
-}
-
 template <typename T, int D, int MAPS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const Params p) {
   constexpr int W = D / MAPS;                 // width of one map's queries and keys

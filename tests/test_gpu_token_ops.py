@@ -172,6 +172,8 @@ BF, FP = torch.bfloat16, torch.float32
     dict(b=2, sq=200, sk=64, h=2, hk=1, causal=True),                                  # the first 136 rows see nothing
     dict(b=2, sq=96, sk=96, h=2, hk=2, causal=True, kv_len=[96, 31], start=0, buckets=4, max_distance=3),
     dict(b=1, sq=64, sk=257, h=3, hk=1, scale=0.31),
+    dict(b=2, sq=70, sk=70, h=2, hk=2, causal=True, scale=-0.2, kv_len=[70, 44], start=0),
+    dict(b=1, sq=70, sk=100, h=1, hk=1, causal=True, scale=0.0, buckets=8, max_distance=10),
 ])
 def test_attention_and_gradients(maps, d, dtype, shape):
     s = dict(shape)
