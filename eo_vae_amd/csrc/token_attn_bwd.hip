@@ -26,28 +26,57 @@ namespace {
 // a wave's score gradients by diagonal: 64 rows (63 distances) of 32 queries, 4 floats apart from the next row's banks
 constexpr int SCR = 36, SCR_FLOATS = 64 * SCR;
 
-template <typename T, int D, int MAPS>
+// fp32's matrix instructions are 16 times slower than bf16's: with fewer blocks of 128 rows than the chip has CUs, a call is a
+// handful of long chains of them.  SPLIT (fp32 only): a block owns 32 rows, its four waves share the other side's tiles and add
+// up through LDS at the end, and the tiles' fragments come from memory (their loads hide behind the matrix instructions), so that
+// LDS is free for the sums.
+template <int D> constexpr int meet_bytes() { return 4 * 32 * (D + 4) * 4; }
+
+// the four waves' [32 columns of acc][D] tiles, added in wave order and stored as rows row0 + column < limit
+template <typename T, int D>
+__device__ __forceinline__ void meet_sum(float* meet, const f32x16 (&acc)[D / 32], float scale, T* out, long long ld, int row0, int limit, int wave,
+                                         int lane) {
+  constexpr int MROW = D + 4;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(f32x4*)(meet + (wave * 32 + (lane & 31)) * MROW + 32 * j + 8 * g + 4 * (lane >> 5)) =
+          f32x4{acc[j][4 * g], acc[j][4 * g + 1], acc[j][4 * g + 2], acc[j][4 * g + 3]};
+  __syncthreads();
+  for (int i = 64 * wave + lane; i < 32 * D / 4; i += 256) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    if (row0 + r >= limit) break;
+    f32x4 v = *(const f32x4*)(meet + r * MROW + d);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) v += *(const f32x4*)(meet + (w * 32 + r) * MROW + d);
+    store4(out + (long long)(row0 + r) * ld + d, scale * v[0], scale * v[1], scale * v[2], scale * v[3]);
+  }
+}
+
+template <typename T, int D, int MAPS, bool SPLIT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dq_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
-  constexpr int NT = D <= 64 && TK::ROWS == 64 ? 2 : 1;           // 32-key tiles worked on together, as the registers allow
+  constexpr int NT = !SPLIT && D <= 64 && TK::ROWS == 64 ? 2 : 1, RB = SPLIT ? 32 : 128;           // 32-key tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* tab = (float*)(lds + Stream<T, D>::BYTES);
+  float* tab = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)Stream<T, D>::BYTES));
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach;
   float* diag = tab + ntab + wave * ntab;                        // [4][ntab]: sums of score gradients by distance
   float* scr = tab + 5 * ntab + 3 - (5 * ntab + 3) % 4 + wave * SCR_FLOATS;
-  const int nbh = p.B * p.H, tiles = (p.Sq + 127) / 128;
+  const int nbh = p.B * p.H, tiles = (p.Sq + RB - 1) / RB;
   const int tile = tiles - 1 - (int)blockIdx.x / nbh;
   int b, hk, h;
   split_bh(p, (int)blockIdx.x % nbh, b, hk, h);
-  const int row0 = tile * 128, limit = key_limit(p, b), start = start_of(p, b);
-  const int rlast = min(row0 + 128, p.Sq) - 1;
+  const int row0 = tile * RB, wrow = SPLIT ? 0 : 32 * wave, limit = key_limit(p, b), start = start_of(p, b);
+  const int rlast = min(row0 + RB, p.Sq) - 1;
   int kend = limit;
   if (p.causal) kend = min(kend, start + rlast + 1);
-  const int qrow = row0 + 32 * wave + (lane & 31);
+  const int qrow = row0 + wrow + (lane & 31);
   const bool live = qrow < p.Sq;
-  const int qlo = start + row0 + 32 * wave, qhi = qlo + 31, qpos = start + qrow;
+  const int qlo = start + row0 + wrow, qhi = qlo + 31, qpos = start + qrow;
   const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
   const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qrow * p.qs;
@@ -81,7 +110,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   for (int a = 0; a < MAPS; ++a) {
     const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + qrow;
     lse[a] = live ? p.lse[at] : INFINITY;
-    if (live && half == 0) p.delta[at] = delta[a];
+    if (live && half == 0 && (!SPLIT || wave == 0)) p.delta[at] = delta[a];
   }
   if (p.bk.n) {
     fill_bias(p, tab, h, tid, 256);
@@ -99,107 +128,127 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) x[a] = m[a] = xl[a] = xr[a] = ml[a] = mr[a] = 0.f;
   const bool sums = p.part || p.lam_part;
-  Stream<T, D> kv(lds);
-  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
-  for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
-    kv.arrive();
-    if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, limit, tid);
-    char *lk = kv.a(), *lv = kv.b();
-#pragma unroll 1
-    for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT) {
-      const int key0 = k0 + 32 * t0, klast = key0 + 32 * NT - 1;
-      if (key0 >= kend || (p.causal && key0 > qhi)) continue;
-      const bool whole = klast < limit && (!p.causal || klast <= qlo);
-      const float* tb = tab + (reach + PAD) + key0 - qpos + 4 * half;
-      float far = 0.f;
-      int side = 0;
-      bool near = false;
-      if (p.bk.n) {
-        if (klast - qlo <= -reach) far = tab[PAD], side = -1;
-        else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
-        else near = true;
-      }
-      f32x16 da[NT];
+  // 32 NT keys from position key0 on, their fragments from ka and va
+  const auto work = [&](const auto& ka, const auto& va, int key0) __attribute__((always_inline)) {
+    const int klast = key0 + 32 * NT - 1;
+    if (p.causal && key0 > qhi) return;
+    const bool whole = klast < limit && (!p.causal || klast <= qlo);
+    const float* tb = tab + (reach + PAD) + key0 - qpos + 4 * half;
+    float far = 0.f;
+    int side = 0;
+    bool near = false;
+    if (p.bk.n) {
+      if (klast - qlo <= -reach) far = tab[PAD], side = -1;
+      else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
+      else near = true;
+    }
+    f32x16 da[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      da[t] = zero16();
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) da[t] = mma(va.frag(32 * t, i), gf[i], da[t]);
+    }
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      f32x16 s[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        da[t] = zero16();
+        s[t] = zero16();
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) da[t] = mma(TK::frag(lv, 32 * (t0 + t), i, lane), gf[i], da[t]);
+        for (int i = 0; i < W / 16; ++i) s[t] = mma(ka.frag(32 * t, a * (W / 16) + i), qf[a * (W / 16) + i], s[t]);
+      }
+      float cc = c, off = far - lse[a];
+      if (near || !whole) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, near ? tb[32 * t + 8 * (r >> 2) + (r & 3)] : far);
+        if (!whole) {
+          const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * t + 8 * (r >> 2) + (r & 3) > last) s[t][r] = -INFINITY;
+        }
+        cc = 1.f;
+        off = -lse[a];
       }
 #pragma unroll
-      for (int a = 0; a < MAPS; ++a) {
-        f32x16 s[NT];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = exp2_(fmaf(s[t][r], cc, off));
+      if (sums) {
+        float xs = 0.f, ms = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            xs = fmaf(s[t][r], da[t][r], xs);
+            ms += s[t][r];
+          }
+        x[a] += xs, m[a] += ms;
+        if (side < 0) xl[a] += xs, ml[a] += ms;
+        if (side > 0) xr[a] += xs, mr[a] += ms;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] *= (a == 0 ? da[t][r] : -lam * da[t][r]) - delta[a];
+      if (p.part && !side) {
+        // [distance key - query + 31][query]: a lane writes its query's column, then lane l sums row l (63 of them); what lies
+        // outside the 32 x 32 tile stays zero from the start
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          s[t] = zero16();
+          float* at = scr + (31 - (lane & 31) + 4 * half) * SCR + (lane & 31);
 #pragma unroll
-          for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, 32 * (t0 + t), a * (W / 16) + i, lane), qf[a * (W / 16) + i], s[t]);
+          for (int r = 0; r < 16; ++r) at[(8 * (r >> 2) + (r & 3)) * SCR] = s[t][r];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 8; ++q) sum += *(const f32x4*)(scr + lane * SCR + 4 * q);
+          if (lane < 63) diag[(reach + PAD) + key0 + 32 * t - qlo + lane - 31] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        float cc = c, off = far - lse[a];
-        if (near || !whole) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, near ? tb[32 * t + 8 * (r >> 2) + (r & 3)] : far);
-          if (!whole) {
-            const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                if (32 * t + 8 * (r >> 2) + (r & 3) > last) s[t][r] = -INFINITY;
-          }
-          cc = 1.f;
-          off = -lse[a];
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = exp2_(fmaf(s[t][r], cc, off));
-        if (sums) {
-          float xs = 0.f, ms = 0.f;
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              xs = fmaf(s[t][r], da[t][r], xs);
-              ms += s[t][r];
-            }
-          x[a] += xs, m[a] += ms;
-          if (side < 0) xl[a] += xs, ml[a] += ms;
-          if (side > 0) xr[a] += xs, mr[a] += ms;
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] *= (a == 0 ? da[t][r] : -lam * da[t][r]) - delta[a];
-        if (p.part && !side) {
-          // [distance key - query + 31][query]: a lane writes its query's column, then lane l sums row l (63 of them); what lies
-          // outside the 32 x 32 tile stays zero from the start
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float* at = scr + (31 - (lane & 31) + 4 * half) * SCR + (lane & 31);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) at[(8 * (r >> 2) + (r & 3)) * SCR] = s[t][r];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < 8; ++q) sum += *(const f32x4*)(scr + lane * SCR + 4 * q);
-            if (lane < 63) diag[(reach + PAD) + key0 + 32 * t - qlo + lane - 31] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            Frag<T> sf;
-            to_frag(sf, s[t], 8 * u);
-#pragma unroll
-            for (int j = 0; j < W / 32; ++j)
-              acc[a * (W / 32) + j] = mma(TK::frag_t(lk, 32 * (t0 + t) + 16 * u, a * W + 32 * j, lane), sf, acc[a * (W / 32) + j]);
-          }
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> sf;
+          to_frag(sf, s[t], 8 * u);
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j)
+            acc[a * (W / 32) + j] = mma(ka.frag_t(32 * t + 16 * u, a * W + 32 * j), sf, acc[a * (W / 32) + j]);
+        }
+    }
+  };
+  if constexpr (SPLIT) {
+    for (int k0 = 32 * wave; k0 < kend; k0 += 128) work(InMemory{kb, p.ks, k0, limit, lane}, InMemory{vb, p.vs, k0, limit, lane}, k0);
+  } else {
+    Stream<T, D> kv(lds);
+    if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
+    for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
+      kv.arrive();
+      if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, limit, tid);
+#pragma unroll 1
+      for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
+        if (k0 + 32 * t0 < kend) work(Staged<T, D>{kv.a(), 32 * t0, lane}, Staged<T, D>{kv.b(), 32 * t0, lane}, k0 + 32 * t0);
+    }
+  }
+  if constexpr (SPLIT) {
+    // the waves' sums over their keys: statistics into every wave, the output tile through the same LDS
+    float* st = (float*)lds;
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      float* v[6] = {&x[a], &m[a], &xl[a], &xr[a], &ml[a], &mr[a]};
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 6; ++i) st[(wave * 6 + i) * 64 + lane] = *v[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 6; ++i) *v[i] = (st[i * 64 + lane] + st[(6 + i) * 64 + lane]) + (st[(12 + i) * 64 + lane] + st[(18 + i) * 64 + lane]);
     }
   }
 #pragma unroll
@@ -211,7 +260,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
     far_l += w * (xl[a] - x[a] * ml[a]);        // both halves: the sum over the wave adds their keys
     far_r += w * (xr[a] - x[a] * mr[a]);
   }
-  if (live) {
+  if constexpr (SPLIT) {
+    if (wave) far_l = far_r = 0.f;                               // the statistics are the same in every wave
+    meet_sum<T, D>((float*)lds, acc, p.scale, (T*)p.dq + ((size_t)b * p.Sq * p.H + h) * D, (long long)p.H * D, row0, p.Sq, wave, lane);
+  } else if (live) {
     T* dq = (T*)p.dq + orow;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
@@ -257,7 +309,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   }
   if constexpr (MAPS == 2) {
     if (p.lam_part) {
-      const float xs = wave_sum(half == 0 ? x[1] : 0.f);
+      const float xs = wave_sum(half == 0 && (!SPLIT || wave == 0) ? x[1] : 0.f);
       __shared__ float lams[4];
       if (lane == 0) lams[wave] = xs;
       __syncthreads();
@@ -266,20 +318,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   }
 }
 
-template <typename T, int D, int MAPS>
+template <typename T, int D, int MAPS, bool SPLIT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_dkv_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
-  constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1;     // 32-query tiles worked on together, as the registers allow
+  constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1, KB = SPLIT ? 32 : 128, STEP = SPLIT ? 32 : TK::ROWS;     // 32-query tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // two of [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it)
-  float* rows2 = (float*)(lds + Stream<T, D>::BYTES);
-  float* tab = rows2 + 2 * MAPS * 4 * TILE;
+  // [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it); one set in use
+  // while the next is written, or one for each wave
+  float* rows2 = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)Stream<T, D>::BYTES));
+  float* tab0 = rows2 + (SPLIT ? 4 : 2) * MAPS * 4 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
-  const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * 128, b = j0 / p.Hkv, hk = j0 % p.Hkv;
+  float* tab = tab0 + (SPLIT && p.bk.n ? wave * (2 * (reach + PAD) + 1) : 0);
+  const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * KB, b = j0 / p.Hkv, hk = j0 % p.Hkv;
   const int limit = key_limit(p, b), start = start_of(p, b);
-  const int krow = kblock + 32 * wave + (lane & 31), klo = kblock + 32 * wave, khi = klo + 31;
+  const int klo = kblock + (SPLIT ? 0 : 32 * wave), krow = klo + (lane & 31), khi = klo + 31;
   const bool live = krow < limit;
   const T* kp = (const T*)p.k + b * p.kb + hk * p.kh + (long long)krow * p.ks;
   const T* vp = (const T*)p.v + b * p.vb + hk * p.vh + (long long)krow * p.vs;
@@ -300,130 +354,169 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   }
   const float c = positive_scale(p.scale, kf);
   int first = 0;                                                  // first query row that sees a key of this block
-  if (p.causal) first = max(0, kblock - start) / TK::ROWS * TK::ROWS;
-  const int per = kblock < limit && first < p.Sq ? (p.Sq - first + TK::ROWS - 1) / TK::ROWS : 0, total = per * G;
-  Stream<T, D> qg(lds);
-  float rl[MAPS], rd[MAPS];
-  const auto fetch = [&](int it) {
-    const int h = hk * G + it / per, q0 = first + it % per * TK::ROWS;
-    qg.next((const T*)p.q + b * p.qb + h * p.qh, p.qs, (const T*)p.d_o + ((size_t)b * p.Sq * p.H + h) * D, (long long)p.H * D, q0, p.Sq, tid);
-    if (tid < TK::ROWS)
+  if (p.causal) first = max(0, kblock - start) / STEP * STEP;
+  const int per = kblock < limit && first < p.Sq ? (p.Sq - first + STEP - 1) / STEP : 0, total = per * G;
+  float rl[MAPS], rd[MAPS], lam = 0.f, far_l = 0.f, far_r = 0.f;
+  // lse and delta of STEP rows from q0 on, one row per thread of `t`
+  const auto fetch_rows = [&](int h, int q0, int t) {
+    if (t < STEP)
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
-        const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + q0 + tid;
-        rl[a] = q0 + tid < p.Sq ? p.lse[at] : INFINITY;
-        rd[a] = q0 + tid < p.Sq ? p.delta[at] : 0.f;
+        const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + q0 + t;
+        rl[a] = q0 + t < p.Sq ? p.lse[at] : INFINITY;
+        rd[a] = q0 + t < p.Sq ? p.delta[at] : 0.f;
       }
   };
-  if (total > 0) fetch(0);
-  float lam = 0.f, far_l = 0.f, far_r = 0.f;
-  for (int it = 0; it < total; ++it) {
-    const int h = hk * G + it / per, q0 = first + it % per * TK::ROWS;
-    float* rows = rows2 + (it & 1) * MAPS * 4 * TILE;            // written while other waves may still read the other one
-    if (it % per == 0) {                                           // a head begins
-      if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
-      if (p.bk.n) {
-        __syncthreads();
-        fill_bias(p, tab, h, tid, 256);
-        __syncthreads();
-        far_l = tab[PAD];
-        far_r = tab[2 * (reach + PAD)];
-      }
-    }
-    if (tid < TK::ROWS)
+  const auto put_rows = [&](float* rows, int t) {
+    if (t < STEP)
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
-        float* at = rows + a * 4 * TILE + tid;
+        float* at = rows + a * 4 * TILE + t;
         at[0] = rd[a];
         at[TILE] = -rl[a];
         at[2 * TILE] = far_l - rl[a];
         at[3 * TILE] = far_r - rl[a];
       }
-    qg.arrive();
-    char *lq = qg.a(), *lg = qg.b();
-    if (it + 1 < total) fetch(it + 1);
-#pragma unroll 1
-    for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT) {
-      const int r0 = q0 + 32 * t0, qlo = start + r0, qhi = qlo + 32 * NT - 1;
-      if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) continue;
-      const bool whole = khi < limit && (!p.causal || khi <= qlo);
-      const float* tb = tab + (reach + PAD) + krow - qlo - 4 * half;
-      int offs = TILE;                                                 // which of a row's offsets
-      bool near = false;
-      if (p.bk.n) {
-        if (khi - qlo <= -reach) offs = 2 * TILE;
-        else if (klo - qhi >= reach) offs = 3 * TILE;
-        else near = true;
-      }
-      f32x16 da[NT], mix[NT];
+  };
+  // 32 NT queries from row r0 on, their fragments from qa and ga, their offsets at `rows`
+  const auto work = [&](const auto& qa, const auto& ga, const float* rows, int r0) __attribute__((always_inline)) {
+    const int qlo = start + r0, qhi = qlo + 32 * NT - 1;
+    if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) return;
+    const bool whole = khi < limit && (!p.causal || khi <= qlo);
+    const float* tb = tab + (reach + PAD) + krow - qlo - 4 * half;
+    int offs = TILE;                                                 // which of a row's offsets
+    bool near = false;
+    if (p.bk.n) {
+      if (khi - qlo <= -reach) offs = 2 * TILE;
+      else if (klo - qhi >= reach) offs = 3 * TILE;
+      else near = true;
+    }
+    f32x16 da[NT], mix[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      da[t] = zero16();
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        da[t] = mma(ga.frag(32 * t, i), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da[t]);
+    }
+#pragma unroll
+    for (int a = 0; a < MAPS; ++a) {
+      f32x16 s[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        da[t] = zero16();
+        s[t] = zero16();
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          da[t] = mma(TK::frag(lg, 32 * (t0 + t), i, lane), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da[t]);
+        for (int i = 0; i < W / 16; ++i) s[t] = mma(qa.frag(32 * t, a * (W / 16) + i), kf[a * (W / 16) + i], s[t]);
       }
-#pragma unroll
-      for (int a = 0; a < MAPS; ++a) {
-        f32x16 s[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s[t] = zero16();
-#pragma unroll
-          for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lq, 32 * (t0 + t), a * (W / 16) + i, lane), kf[a * (W / 16) + i], s[t]);
-        }
-        const float* ls = rows + a * 4 * TILE + 32 * t0 + 4 * half;
-        float cc = c;
-        if (near) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, tb[-(32 * t + 8 * (r >> 2) + (r & 3))]);
-          cc = 1.f;
-        }
-        if (!whole) {       // first query that sees this key
-          const int first = krow >= limit ? 0x7fffffff : (p.causal ? krow - qlo - 4 * half : -0x7fffffff);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * t + 8 * (r >> 2) + (r & 3) < first) s[t][r] = -INFINITY;
-        }
+      const float* ls = rows + a * 4 * TILE + 4 * half;
+      float cc = c;
+      if (near) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4 nl = *(const f32x4*)(ls + offs + 32 * t + 8 * g), dl = *(const f32x4*)(ls + 32 * t + 8 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 4 * g + e;
-              const float x = exp2_(fmaf(s[t][r], cc, nl[e]));
-              if (a == 0) mix[t][r] = x;
-              else mix[t][r] = fmaf(-lam, x, mix[t][r]);
-              s[t][r] = x * ((a == 0 ? da[t][r] : -lam * da[t][r]) - dl[e]);
-            }
-          }
+          for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, tb[-(32 * t + 8 * (r >> 2) + (r & 3))]);
+        cc = 1.f;
+      }
+      if (!whole) {       // first query that sees this key
+        const int first = krow >= limit ? 0x7fffffff : (p.causal ? krow - qlo - 4 * half : -0x7fffffff);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            Frag<T> sf;
-            to_frag(sf, s[t], 8 * u);
-#pragma unroll
-            for (int j = 0; j < W / 32; ++j)
-              dk[a * (W / 32) + j] = mma(TK::frag_t(lq, 32 * (t0 + t) + 16 * u, a * W + 32 * j, lane), sf, dk[a * (W / 32) + j]);
-          }
+          for (int r = 0; r < 16; ++r)
+            if (32 * t + 8 * (r >> 2) + (r & 3) < first) s[t][r] = -INFINITY;
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          Frag<T> pf;
-          to_frag(pf, mix[t], 8 * u);
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 nl = *(const f32x4*)(ls + offs + 32 * t + 8 * g), dl = *(const f32x4*)(ls + 32 * t + 8 * g);
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) dv[j] = mma(TK::frag_t(lg, 32 * (t0 + t) + 16 * u, 32 * j, lane), pf, dv[j]);
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            const float x = exp2_(fmaf(s[t][r], cc, nl[e]));
+            if (a == 0) mix[t][r] = x;
+            else mix[t][r] = fmaf(-lam, x, mix[t][r]);
+            s[t][r] = x * ((a == 0 ? da[t][r] : -lam * da[t][r]) - dl[e]);
+          }
+        }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> sf;
+          to_frag(sf, s[t], 8 * u);
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j)
+            dk[a * (W / 32) + j] = mma(qa.frag_t(32 * t + 16 * u, a * W + 32 * j), sf, dk[a * (W / 32) + j]);
         }
     }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Frag<T> pf;
+        to_frag(pf, mix[t], 8 * u);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) dv[j] = mma(ga.frag_t(32 * t + 16 * u, 32 * j), pf, dv[j]);
+      }
+  };
+  const T* q_of = (const T*)p.q + b * p.qb;
+  const T* g_of = (const T*)p.d_o + (size_t)b * p.Sq * p.H * D;
+  if constexpr (SPLIT) {
+    float* rows = rows2 + wave * MAPS * 4 * TILE;
+    int held = -1;
+    for (int it = wave; it < total; it += 4) {
+      const int h = hk * G + it / per, q0 = first + it % per * STEP;
+      fetch_rows(h, q0, lane);
+      if (h != held) {
+        held = h;
+        if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+        if (p.bk.n) {
+          fill_bias(p, tab, h, lane, 64);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          far_l = tab[PAD];
+          far_r = tab[2 * (reach + PAD)];
+        }
+      }
+      put_rows(rows, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      work(InMemory{q_of + h * p.qh, p.qs, q0, p.Sq, lane}, InMemory{g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, lane}, rows, q0);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  } else {
+    Stream<T, D> qg(lds);
+    const auto fetch = [&](int it) {
+      const int h = hk * G + it / per, q0 = first + it % per * STEP;
+      qg.next(q_of + h * p.qh, p.qs, g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, tid);
+      fetch_rows(h, q0, tid);
+    };
+    if (total > 0) fetch(0);
+    for (int it = 0; it < total; ++it) {
+      const int h = hk * G + it / per, q0 = first + it % per * STEP;
+      float* rows = rows2 + (it & 1) * MAPS * 4 * TILE;          // written while other waves may still read the other one
+      if (it % per == 0) {                                         // a head begins
+        if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+        if (p.bk.n) {
+          __syncthreads();
+          fill_bias(p, tab, h, tid, 256);
+          __syncthreads();
+          far_l = tab[PAD];
+          far_r = tab[2 * (reach + PAD)];
+        }
+      }
+      put_rows(rows, tid);
+      qg.arrive();
+      if (it + 1 < total) fetch(it + 1);
+#pragma unroll 1
+      for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
+        work(Staged<T, D>{qg.a(), 32 * t0, lane}, Staged<T, D>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0);
+    }
+  }
+  if constexpr (SPLIT) {
+    const long long ld = (long long)p.Hkv * D;
+    meet_sum<T, D>((float*)lds, dk, p.scale, (T*)p.dk + ((size_t)b * p.Sk * p.Hkv + hk) * D, ld, klo, p.Sk, wave, lane);
+    meet_sum<T, D>((float*)lds, dv, 1.f, (T*)p.dv + ((size_t)b * p.Sk * p.Hkv + hk) * D, ld, klo, p.Sk, wave, lane);
+    return;
   }
   if (krow < p.Sk) {
     const size_t at = (((size_t)b * p.Sk + krow) * p.Hkv + hk) * D;
@@ -460,9 +553,17 @@ struct Sizes {
   size_t delta, part, lam;      // floats
   int slots;
 };
-Sizes sizes_of(const Params& p, int maps, bool dbias, bool dlam) {
+constexpr int CUS = 256;
+bool split_rows(const eovae_token_attention* d) {
+  return d->dtype == EOVAE_F32 && (long long)d->batch * d->heads * ((d->sq + 127) / 128) < CUS;
+}
+bool split_keys(const eovae_token_attention* d) {
+  return d->dtype == EOVAE_F32 && (long long)d->batch * d->kv_heads * ((d->sk + 127) / 128) < CUS;
+}
+Sizes sizes_of(const Params& p, const eovae_token_attention* d, bool dbias, bool dlam) {
   Sizes s;
-  s.slots = p.B * ((p.Sq + 127) / 128);
+  const int maps = d->maps, rb = split_rows(d) ? 32 : 128;
+  s.slots = p.B * ((p.Sq + rb - 1) / rb);
   s.delta = ((size_t)p.B * p.H * maps * p.Sq + 3) & ~(size_t)3;
   s.part = dbias ? ((size_t)s.slots * p.H * p.bk.n + 3) & ~(size_t)3 : 0;
   s.lam = dlam ? (size_t)s.slots * p.H : 0;
@@ -471,7 +572,7 @@ Sizes sizes_of(const Params& p, int maps, bool dbias, bool dlam) {
 
 template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_attention* d, hipStream_t st) {
   const char* who = "token_attention_bwd";
-  const Sizes s = sizes_of(p, MAPS, d->dbias, d->dlam);
+  const Sizes s = sizes_of(p, d, d->dbias, d->dlam);
   const size_t need = 4 * (s.delta + s.part + s.lam);
   EOVAE_CHECK_ARG(d->ws && d->ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", who, d->ws_bytes, need);
   p.delta = (float*)d->ws;
@@ -479,9 +580,22 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
   if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
   const size_t tiles = (size_t)Stream<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
   const size_t sums = d->dbias ? 4 * tab + 16 + 4 * 4 * SCR_FLOATS : 0;
-  int rc = launch(attn_dq_kernel<T, D, MAPS>, (size_t)((p.Sq + 127) / 128) * p.B * p.H, 256, tiles + tab + sums, p, st, who);
-  if (rc) return rc;
-  rc = launch(attn_dkv_kernel<T, D, MAPS>, (size_t)((p.Sk + 127) / 128) * p.B * p.Hkv, 256, tiles + tab + 2 * 4 * MAPS * 4 * TILE, p, st, who);
+  const size_t rows = 4 * MAPS * 4 * TILE;
+  int rc = EOVAE_OK;
+  const auto dq = [&](auto kernel, int rb, size_t head) {
+    return launch(kernel, (size_t)((p.Sq + rb - 1) / rb) * p.B * p.H, 256, head + tab + sums, p, st, who);
+  };
+  const auto dkv = [&](auto kernel, int kb, size_t head, int copies) {
+    return launch(kernel, (size_t)((p.Sk + kb - 1) / kb) * p.B * p.Hkv, 256, head + copies * rows + (copies == 4 ? 4 : 1) * tab, p, st, who);
+  };
+  if constexpr (sizeof(T) == 4) {
+    const size_t meet = meet_bytes<D>();
+    rc = split_rows(d) ? dq(attn_dq_kernel<T, D, MAPS, true>, 32, meet) : dq(attn_dq_kernel<T, D, MAPS, false>, 128, tiles);
+    if (rc == EOVAE_OK) rc = split_keys(d) ? dkv(attn_dkv_kernel<T, D, MAPS, true>, 32, meet, 4) : dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, tiles, 2);
+  } else {
+    rc = dq(attn_dq_kernel<T, D, MAPS, false>, 128, tiles);
+    if (rc == EOVAE_OK) rc = dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, tiles, 2);
+  }
   if (rc) return rc;
   const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);
   if (outs == 0) return EOVAE_OK;
@@ -500,7 +614,7 @@ size_t eovae_token_attention_workspace(const eovae_token_attention* d, int backw
   Params p;
   if (make_params(d, p, "token_attention_workspace", 0)) return 0;
   if (!backward) return tok_fwd_workspace(d, p);
-  const Sizes s = sizes_of(p, d->maps, d->bias != nullptr, d->maps == 2);
+  const Sizes s = sizes_of(p, d, d->bias != nullptr, d->maps == 2);
   return 4 * (s.delta + s.part + s.lam);
 }
 int eovae_token_attention_bwd(const eovae_token_attention* d, void* stream) {

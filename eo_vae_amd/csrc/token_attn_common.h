@@ -189,6 +189,33 @@ template <typename T, int D> struct Stream {
   }
 };
 
+// Where a 32-row tile's fragments come from: a staged tile, or (fp32) memory itself, rows at and behind `limit` as row limit - 1
+template <typename T, int D> struct Staged {
+  char* lds;
+  int row, lane;
+  __device__ __forceinline__ Frag<T> frag(int r, int s) const { return Tile<T, D>::frag(lds, row + r, s, lane); }
+  __device__ __forceinline__ Frag<T> frag_t(int r, int col) const { return Tile<T, D>::frag_t(lds, row + r, col, lane); }
+};
+struct InMemory {
+  const float* base;
+  long long stride;
+  int row, limit, lane;
+  __device__ __forceinline__ const float* at(int r) const { return base + (long long)(row + r < limit ? row + r : limit - 1) * stride; }
+  __device__ __forceinline__ Frag<float> frag(int r, int s) const {
+    const float* p = at(r + (lane & 31)) + 16 * s + 8 * (lane >> 5);
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+    Frag<float> f;
+    f.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return f;
+  }
+  __device__ __forceinline__ Frag<float> frag_t(int r, int col) const {
+    Frag<float> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.x[i] = at(r + 4 * (lane >> 5) + (i & 3) + 8 * (i >> 2))[col + (lane & 31)];
+    return f;
+  }
+};
+
 // fragment of a row straight from global memory (row < limit, else zero)
 template <typename T> __device__ __forceinline__ Frag<T> frag_global(const T* row, int s, int lane, bool ok) {
   Frag<T> f;

@@ -4,9 +4,9 @@
 // maximum and sum of every row's softmax; a lane owns ONE query (its column of S^T = K Q^T), so the statistics are plain
 // registers and the other half of a column is one cross-lane exchange away.  Two maps: waves 0, 1 hold map 0, waves 2, 3
 // map 1 of the same rows (same K / V tiles, half of K's columns each) and meet once at the end.
-// Step form (few rows per key head, e.g. single tokens against a cache): the rows are the query heads that share one key
-// head times the query tokens (<= 32 per block), the four waves take different keys, the key axis is also split over blocks,
-// and a second kernel joins the partial sums.
+// Step form (few rows per key head, e.g. single tokens against a cache, or a call too small to fill the chip): the rows are the
+// query heads that share one key head times the query tokens, 32 of them to a block, the four waves take different keys, the
+// key axis is also split over blocks where it is long, and then a second kernel joins the partial sums.
 #include <math.h>
 #include "token_attn_common.h"
 
@@ -14,7 +14,9 @@ using namespace tok;
 
 namespace {
 
+constexpr int CUS = 256;
 constexpr int STEP_BLOCKS = 1024;      // blocks that a step-form call is split into
+constexpr int SPLIT_KEYS = 512;        // fewest keys of a split where a call has more than 32 rows per key head
 
 // Scores of one wave's 32 queries against 32 NT keys, turned into probabilities in place (relative to 2^m, not normalised);
 // returns the factor by which the wave's earlier sums have to be multiplied (`moved`: whether any lane's differs from 1).
@@ -224,8 +226,12 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   const bool live = row < rows;
   const int g = live ? row / p.Sq : 0, qi = live ? row % p.Sq : 0, h = hk * G + g;
   const int limit = key_limit(p, b), start = start_of(p, b), qpos = start + qi;
+  // positions of the block's first and last query (all of them where its rows reach into a second head)
+  const int r_last = min(rows, rb * 32 + 32) - 1;
+  const bool one = rb * 32 / p.Sq == r_last / p.Sq;
+  const int qlo = start + (one ? rb * 32 % p.Sq : 0), qhi = start + (one ? r_last % p.Sq : p.Sq - 1);
   int kend = limit;
-  if (p.causal) kend = min(kend, start + p.Sq);
+  if (p.causal) kend = min(kend, qhi + 1);
   const int k_lo = split * p.chunk, k_hi = min(kend, k_lo + p.chunk);
   const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
@@ -272,9 +278,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
     } else {
       wait_dma<0>();
     }
-    const bool near = p.bk.n && k0 + 31 - start > -reach && k0 - (start + p.Sq - 1) < reach;
-    const bool whole = k0 + 31 < k_hi && (!p.causal || k0 + 31 <= start);
-    const float far = k0 + 31 - start <= -reach ? far_l : far_r;
+    const bool near = p.bk.n && k0 + 31 - qlo > -reach && k0 - qhi < reach;
+    const bool whole = k0 + 31 < k_hi && (!p.causal || k0 + 31 <= qlo);
+    const float far = k0 + 31 - qlo <= -reach ? far_l : far_r;
     f32x16 s[MAPS];
     float cc = c, off = far, al[MAPS];
     bool up = false;
@@ -348,7 +354,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   constexpr int MROW = D + 4;
   float* meet = (float*)lds;
   float* stat = meet + WAVES * 32 * MROW;
-  float* out = p.part + (size_t)blockIdx.x * part_floats<D, MAPS>();
+  float* part = p.part + (size_t)blockIdx.x * part_floats<D, MAPS>();
+  constexpr int ITEMS = 32 * D / 4 / (64 * WAVES);             // 4-column pieces of the [32][D] tile per thread
+  f32x4 first[ITEMS];
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
     __syncthreads();
@@ -367,9 +375,10 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
           *(f32x4*)(meet + (wave * 32 + col) * MROW + 32 * i + 8 * q + 4 * half) = v;
         }
     __syncthreads();
-    for (int i = tid; i < 32 * D / 4; i += 64 * WAVES) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      if (rb * 32 + r >= rows) break;
+#pragma unroll
+    for (int e = 0; e < ITEMS; ++e) {
+      const int i = tid + 64 * WAVES * e, r = i / (D / 4), d = 4 * (i % (D / 4)), at = rb * 32 + r;
+      if (at >= rows) continue;
       float mm = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, stat[(w * 32 + r) * 2]);
@@ -382,11 +391,29 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
         ls += f * stat[(w * 32 + r) * 2 + 1];
         sum += f * *(const f32x4*)(meet + (w * 32 + r) * MROW + d);
       }
-      *(f32x4*)(out + (a * 32 + r) * D + d) = sum;
-      if (d == 0) {
-        out[MAPS * 32 * D + (a * 32 + r) * 2] = mm;
-        out[MAPS * 32 * D + (a * 32 + r) * 2 + 1] = ls;
+      if (p.splits > 1) {
+        *(f32x4*)(part + (a * 32 + r) * D + d) = sum;
+        if (d == 0) {
+          part[MAPS * 32 * D + (a * 32 + r) * 2] = mm;
+          part[MAPS * 32 * D + (a * 32 + r) * 2 + 1] = ls;
+        }
+        continue;
       }
+      // the whole key axis in this block: the rows leave from here
+      const int hr = hk * G + at / p.Sq, qr = at % p.Sq;
+      const size_t o_at = (((size_t)b * p.Sq + qr) * p.H + hr) * D + d;
+      sum *= ls > 0.f ? 1.f / ls : 0.f;
+      if (p.lse && d == 0) p.lse[(((size_t)b * p.H + hr) * MAPS + a) * p.Sq + qr] = ls > 0.f ? mm + __builtin_amdgcn_logf(ls) : INFINITY;
+      if (MAPS == 2 && a == 0) {
+        first[e] = sum;
+        continue;
+      }
+      if constexpr (MAPS == 2) {
+        if (p.out2) store4((T*)p.out2 + o_at, sum[0], sum[1], sum[2], sum[3]);
+        const float lam = ldf(p.lam, hr, p.lam_f32);
+        sum = first[e] - lam * sum;
+      }
+      store4((T*)p.out + o_at, sum[0], sum[1], sum[2], sum[3]);
     }
   }
 }
@@ -452,16 +479,17 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   const size_t meet = (size_t)WAVES * 32 * (D + 4) * 4 + WAVES * 32 * 2 * 4;
   r.lds = WAVES * 4 * 32 * (size_t)Tile<T, D>::ROWB + bias;
   if (r.lds < meet) r.lds = meet;
-  r.step = rows <= 32 && r.lds <= 160 * 1024;
-  r.rblocks = (int)((rows + 31) / 32);
+  // Step form: few rows per key head (then only the key axis can fill the chip), or fewer blocks of the row form than CUs
+  r.step = (rows <= 32 || (long long)p.B * p.H * ((p.Sq * (long long)MAPS + 127) / 128) < CUS) && r.lds <= 160 * 1024;
   if (!r.step) return r;
-  const long long base = (long long)p.B * p.Hkv * r.rblocks, most = (p.Sk + KEYS - 1) / KEYS;
+  r.rblocks = (int)((rows + 31) / 32);
+  const long long base = (long long)p.B * p.Hkv * r.rblocks, keys = rows <= 32 ? KEYS : SPLIT_KEYS, most = (p.Sk + keys - 1) / keys;
   long long want = (STEP_BLOCKS + base - 1) / base;
   if (want > most) want = most;
   if (want > MAX_SPLITS) want = MAX_SPLITS;
   r.chunk = (int)(((p.Sk + want - 1) / want + KEYS - 1) / KEYS * KEYS);
   r.splits = (p.Sk + r.chunk - 1) / r.chunk;
-  r.part_bytes = (size_t)base * r.splits * part_floats<D, MAPS>() * 4;
+  r.part_bytes = r.splits > 1 ? (size_t)base * r.splits * part_floats<D, MAPS>() * 4 : 0;
   return r;
 }
 
@@ -471,13 +499,13 @@ template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t w
   const char* who = "token_attention_fwd";
   const Plan r = plan_of<T, D, MAPS>(p);
   if (r.step) {
-    EOVAE_CHECK_ARG(ws && ws_bytes >= r.part_bytes, "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, r.part_bytes);
+    EOVAE_CHECK_ARG(r.part_bytes == 0 || (ws && ws_bytes >= r.part_bytes), "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, r.part_bytes);
     p.part = (float*)ws;
     p.splits = r.splits;
     p.chunk = r.chunk;
     const size_t base = (size_t)p.B * p.Hkv;
     const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 64 * step_waves<T, D>(), r.lds, p, st, who);
-    if (rc) return rc;
+    if (rc || r.splits == 1) return rc;
     return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, 256, 0, p, st, who);
   }
   constexpr int RB = 128 / MAPS;

@@ -131,7 +131,7 @@ def test_the_library_refuses_bad_borders_and_small_workspaces():
     far = (C.c_int * 15)(*range(1020, 1035))
     d = attention_descriptor(bias=1 << 20, buckets=32, borders=C.cast(far, C.c_void_p).value)
     assert lib.eovae_token_attention_fwd(C.byref(d), None) == -1 and b'border' in lib.eovae_last_error()
-    d = attention_descriptor(sq=1)
+    d = attention_descriptor(sq=1, sk=5000)
     need = lib.eovae_token_attention_workspace(C.byref(d), 0)
     assert need > 0
     d.ws, d.ws_bytes = 1 << 20, need - 1
