@@ -56,13 +56,13 @@ __device__ __forceinline__ void meet_sum(float* meet, const f32x16 (&acc)[D / 32
 }
 
 template <typename T, int D, int MAPS, bool SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dq_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const Params p) {
   using TK = Tile<T, D>;
   constexpr int W = D / MAPS;
   constexpr int NT = !SPLIT && D <= 64 && TK::ROWS == 64 ? 2 : 1, RB = SPLIT ? 32 : 128;           // 32-key tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float* tab = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)Stream<T, D>::BYTES));
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int ntab = p.bk.n ? 2 * (p.bk.reach + PAD) + 1 : 0, reach = p.bk.reach;
   float* diag = tab + ntab + wave * ntab;                        // [4][ntab]: sums of score gradients by distance
   float* scr = tab + 5 * ntab + 3 - (5 * ntab + 3) % 4 + wave * SCR_FLOATS;
@@ -297,10 +297,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
       auto lo = [&](int n) { return n <= p.bk.exact ? n : p.bk.border[n - p.bk.exact - 1]; };
       const int a = lo(i), z = i == last ? reach + PAD + 1 : lo(i + 1);    // distances a .. z - 1; behind them the far sums
       float sum = 0.f;
+#pragma unroll 8
       for (int n = a; n < z; ++n) sum += right ? (n > 0 ? mid[n] : 0.f) : mid[-n];
       if (i == last)
         for (int w = 0; w < 4; ++w) sum += fars[2 * w + right];
       if (!p.bk.two_sided && i == 0) {                                     // one-sided: everything ahead is distance 0
+#pragma unroll 8
         for (int n = 1; n <= reach + PAD; ++n) sum += mid[n];
         for (int w = 0; w < 4; ++w) sum += fars[2 * w + 1];
       }
@@ -318,17 +320,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   }
 }
 
+template <typename T, int D, int MAPS> constexpr bool v_in_lds() { return sizeof(T) == 2 && D == 128 && MAPS == 1; }
+template <typename T, int D, int MAPS> constexpr int dkv_head() {
+  return v_in_lds<T, D, MAPS>() ? Stream<T, D, 32>::BYTES + Tile<T, D, 128>::BYTES : Stream<T, D>::BYTES;
+}
+
 template <typename T, int D, int MAPS, bool SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_dkv_kernel(const Params p) {
-  using TK = Tile<T, D>;
+__global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dkv_kernel(const Params p) {
+  // bf16 at 128 columns, one map: two waves per SIMD leave 256 registers each, 160 of them accumulators and keys; the block's values stay in
+  // LDS, and the stream's tiles are half as long, so that two blocks share a CU
+  constexpr bool VLDS = v_in_lds<T, D, MAPS>();
+  using TK = Tile<T, D, VLDS ? 32 : tile_rows<T, D>()>;
+  using VT = Tile<T, D, 128>;
   constexpr int W = D / MAPS;
   constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1, KB = SPLIT ? 32 : 128, STEP = SPLIT ? 32 : TK::ROWS;     // 32-query tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
   // [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it); one set in use
   // while the next is written, or one for each wave
-  float* rows2 = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)Stream<T, D>::BYTES));
+  float* rows2 = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)dkv_head<T, D, MAPS>()));
   float* tab0 = rows2 + (SPLIT ? 4 : 2) * MAPS * 4 * TILE;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   float* tab = tab0 + (SPLIT && p.bk.n ? wave * (2 * (reach + PAD) + 1) : 0);
   const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * KB, b = j0 / p.Hkv, hk = j0 % p.Hkv;
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
   const T* vp = (const T*)p.v + b * p.vb + hk * p.vh + (long long)krow * p.vs;
   // fp32 at 128 columns: keys, values and both accumulators do not fit in 512 registers; the values come from the cache again for
   // every tile (16 KiB against 8192 cycles of matrix instructions)
-  constexpr bool HOLD = sizeof(T) * D <= 256;
+  constexpr bool HOLD = sizeof(T) * D <= 256 && !VLDS;
   Frag<T> kf[D / 16], vf[HOLD ? D / 16 : 1];
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -378,6 +389,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
         at[3 * TILE] = far_r - rl[a];
       }
   };
+  char* vlds = lds + Stream<T, D, TK::ROWS>::BYTES;
+  const auto v_frag = [&](int i) __attribute__((always_inline)) {
+    if constexpr (HOLD) return vf[i];
+    else if constexpr (VLDS) return VT::frag(vlds, 32 * wave, i, lane);
+    else return frag_global(vp, i, lane, live);
+  };
   // 32 NT queries from row r0 on, their fragments from qa and ga, their offsets at `rows`
   const auto work = [&](const auto& qa, const auto& ga, const float* rows, int r0) __attribute__((always_inline)) {
     const int qlo = start + r0, qhi = qlo + 32 * NT - 1;
@@ -391,13 +408,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       else if (klo - qhi >= reach) offs = 3 * TILE;
       else near = true;
     }
-    f32x16 da[NT], mix[NT];
+    f32x16 da[NT], mix[MAPS == 2 ? NT : 1];
+    const auto add_dv = [&](const f32x16 (&w)[NT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Frag<T> pf;
+          to_frag(pf, w[t], 8 * u);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) dv[j] = mma(ga.frag_t(32 * t + 16 * u, 32 * j), pf, dv[j]);
+        }
+    };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       da[t] = zero16();
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
-        da[t] = mma(ga.frag(32 * t, i), HOLD ? vf[HOLD ? i : 0] : frag_global(vp, i, lane, live), da[t]);
+        da[t] = mma(ga.frag(32 * t, i), v_frag(i), da[t]);
     }
 #pragma unroll
     for (int a = 0; a < MAPS; ++a) {
@@ -429,15 +457,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 nl = *(const f32x4*)(ls + offs + 32 * t + 8 * g), dl = *(const f32x4*)(ls + 32 * t + 8 * g);
+          const f32x4 nl = *(const f32x4*)(ls + offs + 32 * t + 8 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            const float x = exp2_(fmaf(s[t][r], cc, nl[e]));
-            if (a == 0) mix[t][r] = x;
-            else mix[t][r] = fmaf(-lam, x, mix[t][r]);
-            s[t][r] = x * ((a == 0 ? da[t][r] : -lam * da[t][r]) - dl[e]);
-          }
+          for (int e = 0; e < 4; ++e) s[t][4 * g + e] = exp2_(fmaf(s[t][4 * g + e], cc, nl[e]));
+        }
+      if constexpr (MAPS == 2) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mix[t][r] = a == 0 ? s[t][r] : fmaf(-lam, s[t][r], mix[t][r]);
+        if (a == 1) add_dv(mix);
+      } else {
+        add_dv(s);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 dl = *(const f32x4*)(ls + 32 * t + 8 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][4 * g + e] *= (a == 0 ? da[t][4 * g + e] : -lam * da[t][4 * g + e]) - dl[e];
         }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -450,15 +489,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
             dk[a * (W / 32) + j] = mma(qa.frag_t(32 * t + 16 * u, a * W + 32 * j), sf, dk[a * (W / 32) + j]);
         }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        Frag<T> pf;
-        to_frag(pf, mix[t], 8 * u);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) dv[j] = mma(ga.frag_t(32 * t + 16 * u, 32 * j), pf, dv[j]);
-      }
   };
   const T* q_of = (const T*)p.q + b * p.qb;
   const T* g_of = (const T*)p.d_o + (size_t)b * p.Sq * p.H * D;
@@ -484,12 +514,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   } else {
-    Stream<T, D> qg(lds);
+    Stream<T, D, TK::ROWS> qg(lds);
     const auto fetch = [&](int it) {
       const int h = hk * G + it / per, q0 = first + it % per * STEP;
       qg.next(q_of + h * p.qh, p.qs, g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, tid);
       fetch_rows(h, q0, tid);
     };
+    if (VLDS && total > 0) VT::dma((const T*)p.v + b * p.vb + hk * p.vh, p.vs, kblock, limit, vlds, tid);
     if (total > 0) fetch(0);
     for (int it = 0; it < total; ++it) {
       const int h = hk * G + it / per, q0 = first + it % per * STEP;
@@ -509,7 +540,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D <= 64 ? 2 : 1) void attn_d
       if (it + 1 < total) fetch(it + 1);
 #pragma unroll 1
       for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
-        work(Staged<T, D>{qg.a(), 32 * t0, lane}, Staged<T, D>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0);
+        work(Staged<T, D, TK::ROWS>{qg.a(), 32 * t0, lane}, Staged<T, D, TK::ROWS>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0);
     }
   }
   if constexpr (SPLIT) {
@@ -591,10 +622,10 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
   if constexpr (sizeof(T) == 4) {
     const size_t meet = meet_bytes<D>();
     rc = split_rows(d) ? dq(attn_dq_kernel<T, D, MAPS, true>, 32, meet) : dq(attn_dq_kernel<T, D, MAPS, false>, 128, tiles);
-    if (rc == EOVAE_OK) rc = split_keys(d) ? dkv(attn_dkv_kernel<T, D, MAPS, true>, 32, meet, 4) : dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, tiles, 2);
+    if (rc == EOVAE_OK) rc = split_keys(d) ? dkv(attn_dkv_kernel<T, D, MAPS, true>, 32, meet, 4) : dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, dkv_head<T, D, MAPS>(), 2);
   } else {
     rc = dq(attn_dq_kernel<T, D, MAPS, false>, 128, tiles);
-    if (rc == EOVAE_OK) rc = dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, tiles, 2);
+    if (rc == EOVAE_OK) rc = dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, dkv_head<T, D, MAPS>(), 2);
   }
   if (rc) return rc;
   const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);

@@ -40,7 +40,9 @@ __device__ __forceinline__ int bucket_of(const Buckets& t, int rel) {
   int b = n;
   if (n >= t.exact) {
     b = t.exact;
-    for (int i = 0; i < t.nborders; ++i) b += n >= t.border[i] ? 1 : 0;
+    for (int i = 0; i < t.nborders; i += 8)       // border[] is padded with the largest int: eight at a time, one scalar load
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b += n >= t.border[i + j] ? 1 : 0;
   }
   return b + (t.two_sided && rel > 0 ? t.side : 0);
 }
@@ -87,8 +89,10 @@ __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0
 // ---- staged tiles: ROWS rows of D elements, 16-byte chunks, chunk index XORed with swz(row) ----
 // Eight consecutive rows at one chunk index (a fragment read: lanes = rows) fall into eight different 16-byte bank groups,
 // and four consecutive rows times two consecutive chunks (a transposed 16-bit read) cover all 128 bytes once.
-template <typename T, int D> struct Tile {
-  static constexpr int ROWS = sizeof(T) * D > 256 ? 32 : TILE;   // fp32 rows of 128: half, so that two pairs of tiles and the sums fit in LDS
+// default rows; fp32 rows of 128: half, so that two pairs of tiles and the sums fit in LDS
+template <typename T, int D> constexpr int tile_rows() { return sizeof(T) * D > 256 ? 32 : TILE; }
+template <typename T, int D, int R = tile_rows<T, D>()> struct Tile {
+  static constexpr int ROWS = R;
   static constexpr int ROWB = D * (int)sizeof(T);
   static constexpr int CH = ROWB / 16;                       // chunks per row: 4 .. 32
   static constexpr int BYTES = ROWS * ROWB;
@@ -103,7 +107,9 @@ template <typename T, int D> struct Tile {
   // same).  Rows at and behind `limit` (>= 1) become copies of row limit - 1: finite wherever the caller's data is, and never
   // visible.  A block of 256 threads calls; wait_dma<0>() before the barrier that publishes it.
   static __device__ __forceinline__ void dma(const T* base, long long stride, int row0, int limit, const char* lds, int tid) {
-    const int row = tid / CH, col = ((tid % CH) ^ swz(row)) << 4;
+    int row = tid / CH;
+    const int col = ((tid % CH) ^ swz(row)) << 4;
+    asm volatile("" : "+v"(row));               // the 64-bit products below are cheaper than the registers that would keep them
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds +
                                                                        (unsigned)(tid & ~63) * 16u));
     if (row0 + ROWS <= limit) {
@@ -169,8 +175,8 @@ template <typename T, int D> struct Tile {
 // the next pair arrives by DMA while this one is used, one barrier per tile.
 //   next(...)      request a pair of tiles
 //   arrive()       they are in LDS for every wave: a(), b() until the next arrive; the pair before is free
-template <typename T, int D> struct Stream {
-  using TK = Tile<T, D>;
+template <typename T, int D, int R = tile_rows<T, D>()> struct Stream {
+  using TK = Tile<T, D, R>;
   static constexpr int BYTES = 4 * TK::BYTES;
   char* lds;
   int flip;
@@ -190,11 +196,11 @@ template <typename T, int D> struct Stream {
 };
 
 // Where a 32-row tile's fragments come from: a staged tile, or (fp32) memory itself, rows at and behind `limit` as row limit - 1
-template <typename T, int D> struct Staged {
+template <typename T, int D, int R = tile_rows<T, D>()> struct Staged {
   char* lds;
   int row, lane;
-  __device__ __forceinline__ Frag<T> frag(int r, int s) const { return Tile<T, D>::frag(lds, row + r, s, lane); }
-  __device__ __forceinline__ Frag<T> frag_t(int r, int col) const { return Tile<T, D>::frag_t(lds, row + r, col, lane); }
+  __device__ __forceinline__ Frag<T> frag(int r, int s) const { return Tile<T, D, R>::frag(lds, row + r, s, lane); }
+  __device__ __forceinline__ Frag<T> frag_t(int r, int col) const { return Tile<T, D, R>::frag_t(lds, row + r, col, lane); }
 };
 struct InMemory {
   const float* base;
@@ -354,6 +360,7 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   p.scale = d->scale;
   Buckets& t = p.bk;
   t.n = t.side = t.exact = t.nborders = t.reach = t.two_sided = 0;
+  for (int& e : t.border) e = 0x7fffffff;
   if (d->bias) {
     EOVAE_CHECK_ARG(d->buckets >= 2 && d->buckets <= MAX_BUCKETS, "%s: %d buckets (2 .. %d)", who, d->buckets, MAX_BUCKETS);
     t.n = d->buckets;

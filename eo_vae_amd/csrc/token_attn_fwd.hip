@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
   constexpr int RB = 128 / MAPS;              // query rows of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float* tab = (float*)(lds + Stream<T, D>::BYTES);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int map = MAPS == 2 ? wave >> 1 : 0, wrow = 32 * (MAPS == 2 ? (wave & 1) : wave);
   const int nbh = p.B * p.H, tiles = (p.Sq + RB - 1) / RB;
   const int tile = tiles - 1 - (int)blockIdx.x / nbh;      // causal: the longest rows first
@@ -484,7 +484,8 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   if (!r.step) return r;
   r.rblocks = (int)((rows + 31) / 32);
   const long long base = (long long)p.B * p.Hkv * r.rblocks, keys = rows <= 32 ? KEYS : SPLIT_KEYS, most = (p.Sk + keys - 1) / keys;
-  long long want = (STEP_BLOCKS + base - 1) / base;
+  long long want = rows <= 32 ? (STEP_BLOCKS + base - 1) / base : CUS / base;      // many rows: joining costs more than a few idle CUs
+  if (want < 1) want = 1;
   if (want > most) want = most;
   if (want > MAX_SPLITS) want = MAX_SPLITS;
   r.chunk = (int)(((p.Sk + want - 1) / want + KEYS - 1) / KEYS * KEYS);
