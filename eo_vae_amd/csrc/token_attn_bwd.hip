@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   float* tab = tab0 + (SPLIT && p.bk.n ? wave * (2 * (reach + PAD) + 1) : 0);
-  const int j0 = (int)blockIdx.x % n, kblock = ((int)blockIdx.x / n) * KB, b = j0 / p.Hkv, hk = j0 % p.Hkv;
+  const int share = (int)blockIdx.x % p.parts, block = (int)blockIdx.x / p.parts, j0 = block % n, kblock = block / n * KB, b = j0 / p.Hkv, hk = j0 % p.Hkv;
   const int limit = key_limit(p, b), start = start_of(p, b);
   const int klo = kblock + (SPLIT ? 0 : 32 * wave), krow = klo + (lane & 31), khi = klo + 31;
   const bool live = krow < limit;
@@ -520,12 +520,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
       qg.next(q_of + h * p.qh, p.qs, g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, tid);
       fetch_rows(h, q0, tid);
     };
-    if (VLDS && total > 0) VT::dma((const T*)p.v + b * p.vb + hk * p.vh, p.vs, kblock, limit, vlds, tid);
-    if (total > 0) fetch(0);
-    for (int it = 0; it < total; ++it) {
+    // this block's part of the (head, query tile) list
+    const int it0 = (int)((long long)total * share / p.parts), it1 = (int)((long long)total * (share + 1) / p.parts);
+    if (VLDS && it0 < it1) VT::dma((const T*)p.v + b * p.vb + hk * p.vh, p.vs, kblock, limit, vlds, tid);
+    if (it0 < it1) fetch(it0);
+    for (int it = it0; it < it1; ++it) {
       const int h = hk * G + it / per, q0 = first + it % per * STEP;
       float* rows = rows2 + (it & 1) * MAPS * 4 * TILE;          // written while other waves may still read the other one
-      if (it % per == 0) {                                         // a head begins
+      if (it == it0 || it % per == 0) {                             // a head begins
         if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
         if (p.bk.n) {
           __syncthreads();
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
       }
       put_rows(rows, tid);
       qg.arrive();
-      if (it + 1 < total) fetch(it + 1);
+      if (it + 1 < it1) fetch(it + 1);
 #pragma unroll 1
       for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
         work(Staged<T, D, TK::ROWS>{qg.a(), 32 * t0, lane}, Staged<T, D, TK::ROWS>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0);
@@ -556,10 +558,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = 32 * j + 8 * g + 4 * half;
+        if (p.parts > 1) {
+          const size_t pt = (size_t)share * p.B * p.Sk * p.Hkv * D + at + d;
+          store4(p.dk_part + pt, p.scale * dk[j][4 * g], p.scale * dk[j][4 * g + 1], p.scale * dk[j][4 * g + 2], p.scale * dk[j][4 * g + 3]);
+          store4(p.dv_part + pt, dv[j][4 * g], dv[j][4 * g + 1], dv[j][4 * g + 2], dv[j][4 * g + 3]);
+          continue;
+        }
         store4((T*)p.dk + at + d, p.scale * dk[j][4 * g], p.scale * dk[j][4 * g + 1], p.scale * dk[j][4 * g + 2], p.scale * dk[j][4 * g + 3]);
         store4((T*)p.dv + at + d, dv[j][4 * g], dv[j][4 * g + 1], dv[j][4 * g + 2], dv[j][4 * g + 3]);
       }
   }
+}
+
+// dk and dv from their parts, four values per thread, in the parts' order
+template <typename T> __global__ __launch_bounds__(256) void attn_parts_kernel(const Params p, long long n) {
+  const long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  if (i >= n) return;
+  f32x4 a = *(const f32x4*)(p.dk_part + i), b = *(const f32x4*)(p.dv_part + i);
+  for (int k = 1; k < p.parts; ++k) {
+    a += *(const f32x4*)(p.dk_part + k * n + i);
+    b += *(const f32x4*)(p.dv_part + k * n + i);
+  }
+  store4((T*)p.dk + i, a[0], a[1], a[2], a[3]);
+  store4((T*)p.dv + i, b[0], b[1], b[2], b[3]);
 }
 
 // table gradient [n][H] and lambda gradient [H] from the blocks' partial sums; one wave per value, fp64, fixed order
@@ -581,8 +602,8 @@ __global__ __launch_bounds__(64) void attn_fold_kernel(const float* part, const 
 }
 
 struct Sizes {
-  size_t delta, part, lam;      // floats
-  int slots;
+  size_t delta, part, lam, dkv;      // floats; dkv: of each of dk's and dv's parts together
+  int slots, parts;
 };
 constexpr int CUS = 256;
 bool split_rows(const eovae_token_attention* d) {
@@ -597,18 +618,31 @@ Sizes sizes_of(const Params& p, const eovae_token_attention* d, bool dbias, bool
   s.slots = p.B * ((p.Sq + rb - 1) / rb);
   s.delta = ((size_t)p.B * p.H * maps * p.Sq + 3) & ~(size_t)3;
   s.part = dbias ? ((size_t)s.slots * p.H * p.bk.n + 3) & ~(size_t)3 : 0;
-  s.lam = dlam ? (size_t)s.slots * p.H : 0;
+  s.lam = dlam ? ((size_t)s.slots * p.H + 3) & ~(size_t)3 : 0;
+  // Few key heads and a long key axis leave CUs without a block (and, causal, one long row of blocks): the queries are cut into
+  // parts until there are two blocks per CU, and dk, dv are joined from fp32 parts.
+  const long long blocks = (long long)d->batch * d->kv_heads * ((d->sk + 127) / 128), items = (long long)(d->heads / d->kv_heads) * ((d->sq + 127) / 128);
+  long long parts = split_keys(d) || blocks > CUS ? 1 : 2 * CUS / blocks;
+  if (parts > 8) parts = 8;
+  if (parts > items) parts = items;
+  s.parts = (int)parts;
+  s.dkv = parts > 1 ? (size_t)parts * p.B * p.Sk * p.Hkv * d->dim : 0;
   return s;
 }
 
 template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_attention* d, hipStream_t st) {
   const char* who = "token_attention_bwd";
   const Sizes s = sizes_of(p, d, d->dbias, d->dlam);
-  const size_t need = 4 * (s.delta + s.part + s.lam);
+  const size_t need = 4 * (s.delta + s.part + s.lam + 2 * s.dkv);
   EOVAE_CHECK_ARG(d->ws && d->ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", who, d->ws_bytes, need);
   p.delta = (float*)d->ws;
   if (d->dbias) p.part = p.delta + s.delta;
   if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
+  p.parts = s.parts;
+  if (s.parts > 1) {
+    p.dk_part = p.delta + s.delta + s.part + s.lam;
+    p.dv_part = p.dk_part + s.dkv;
+  }
   const size_t tiles = (size_t)Stream<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
   const size_t sums = d->dbias ? 4 * tab + 16 + 4 * 4 * SCR_FLOATS : 0;
   const size_t rows = 4 * MAPS * 4 * TILE;
@@ -617,7 +651,7 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
     return launch(kernel, (size_t)((p.Sq + rb - 1) / rb) * p.B * p.H, 256, head + tab + sums, p, st, who);
   };
   const auto dkv = [&](auto kernel, int kb, size_t head, int copies) {
-    return launch(kernel, (size_t)((p.Sk + kb - 1) / kb) * p.B * p.Hkv, 256, head + copies * rows + (copies == 4 ? 4 : 1) * tab, p, st, who);
+    return launch(kernel, (size_t)((p.Sk + kb - 1) / kb) * p.B * p.Hkv * p.parts, 256, head + copies * rows + (copies == 4 ? 4 : 1) * tab, p, st, who);
   };
   if constexpr (sizeof(T) == 4) {
     const size_t meet = meet_bytes<D>();
@@ -628,6 +662,12 @@ template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_
     if (rc == EOVAE_OK) rc = dkv(attn_dkv_kernel<T, D, MAPS, false>, 128, dkv_head<T, D, MAPS>(), 2);
   }
   if (rc) return rc;
+  if (p.parts > 1) {
+    const long long n = (long long)p.B * p.Sk * p.Hkv * D;
+    EOVAE_CHECK_ARG((n + 1023) / 1024 <= 0x7fffffff, "%s: %lld values of dk", who, n);
+    hipLaunchKernelGGL(attn_parts_kernel<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, p, n);
+    EOVAE_CHECK_LAUNCH(who);
+  }
   const int nb = d->dbias ? p.bk.n : 0, outs = nb + (d->dlam ? 1 : 0);
   if (outs == 0) return EOVAE_OK;
   hipLaunchKernelGGL(attn_fold_kernel, dim3((unsigned)(p.H * outs)), dim3(64), 0, st, p.part, p.lam_part, d->dbias, d->dlam, nb, p.H, s.slots,
@@ -646,7 +686,7 @@ size_t eovae_token_attention_workspace(const eovae_token_attention* d, int backw
   if (make_params(d, p, "token_attention_workspace", 0)) return 0;
   if (!backward) return tok_fwd_workspace(d, p);
   const Sizes s = sizes_of(p, d, d->bias != nullptr, d->maps == 2);
-  return 4 * (s.delta + s.part + s.lam);
+  return 4 * (s.delta + s.part + s.lam + 2 * s.dkv);
 }
 int eovae_token_attention_bwd(const eovae_token_attention* d, void* stream) {
   Params p;

@@ -53,9 +53,10 @@ struct Params {
   void *dq, *dk, *dv;
   const void *bias, *lam;
   const int *kv_len, *q_start;
+  float *dk_part, *dv_part;                   // [parts] of dk and dv in fp32, where a block walks only a part of the queries
   float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain (+inf: nothing visible); delta likewise
   long long qb, qs, qh, kb, ks, kh, vb, vs, vh;   // element strides: batch, token, head
-  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, chunk;
+  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, chunk, parts;
   float scale;
   Buckets bk;
 };
@@ -107,9 +108,9 @@ template <typename T, int D, int R = tile_rows<T, D>()> struct Tile {
   // same).  Rows at and behind `limit` (>= 1) become copies of row limit - 1: finite wherever the caller's data is, and never
   // visible.  A block of 256 threads calls; wait_dma<0>() before the barrier that publishes it.
   static __device__ __forceinline__ void dma(const T* base, long long stride, int row0, int limit, const char* lds, int tid) {
-    int row = tid / CH;
-    const int col = ((tid % CH) ^ swz(row)) << 4;
-    asm volatile("" : "+v"(row));               // the 64-bit products below are cheaper than the registers that would keep them
+    int t = tid;
+    asm volatile("" : "+v"(t));                 // what follows is cheaper than the registers that would keep it from tile to tile
+    const int row = t / CH, col = ((t % CH) ^ swz(row)) << 4;
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds +
                                                                        (unsigned)(tid & ~63) * 16u));
     if (row0 + ROWS <= limit) {
@@ -356,7 +357,7 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   p.vb = d->v_strides[0]; p.vs = d->v_strides[1]; p.vh = d->v_strides[2];
   p.B = d->batch; p.Sq = d->sq; p.Sk = d->sk; p.H = d->heads; p.Hkv = d->kv_heads; p.start = d->start; p.causal = d->causal ? 1 : 0;
   p.bias_f32 = d->bias_dtype == EOVAE_F32; p.lam_f32 = d->lam_dtype == EOVAE_F32;
-  p.splits = 1; p.chunk = 0;
+  p.splits = 1; p.chunk = 0; p.parts = 1; p.dk_part = p.dv_part = nullptr;
   p.scale = d->scale;
   Buckets& t = p.bk;
   t.n = t.side = t.exact = t.nborders = t.reach = t.two_sided = 0;

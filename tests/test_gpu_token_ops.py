@@ -209,6 +209,14 @@ def run_and_check_padded(x, maps, lens, start):
         inside(g, val[n], err[n], n)
 
 
+@pytest.mark.parametrize('maps,d', [(1, 64), (1, 128), (2, 128)])
+@pytest.mark.parametrize('causal', [False, True])
+def test_key_gradients_joined_from_parts(maps, d, causal):
+    """Few key heads: the queries of one key block are walked by several thread blocks."""
+    x = make(1, 333, 210, 6, 1, d, BF, maps, 16, seed=14)
+    run_and_check(x, maps, 40, not causal, causal, start=-100 if causal else None)
+
+
 @pytest.mark.parametrize('maps', [1, 2])
 def test_parameters_in_fp32_beside_bf16_tokens(maps):
     run_and_check(make(2, 50, 50, 2, 2, 64, BF, maps, 32, param=FP), maps)
