@@ -56,7 +56,7 @@ struct Params {
   float *dk_part, *dv_part;                   // [parts] of dk and dv in fp32, where a block walks only a part of the queries
   float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain (+inf: nothing visible); delta likewise
   long long qb, qs, qh, kb, ks, kh, vb, vs, vh;   // element strides: batch, token, head
-  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, chunk, parts;
+  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, parts;
   float scale;
   Buckets bk;
 };
@@ -357,7 +357,7 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   p.vb = d->v_strides[0]; p.vs = d->v_strides[1]; p.vh = d->v_strides[2];
   p.B = d->batch; p.Sq = d->sq; p.Sk = d->sk; p.H = d->heads; p.Hkv = d->kv_heads; p.start = d->start; p.causal = d->causal ? 1 : 0;
   p.bias_f32 = d->bias_dtype == EOVAE_F32; p.lam_f32 = d->lam_dtype == EOVAE_F32;
-  p.splits = 1; p.chunk = 0; p.parts = 1; p.dk_part = p.dv_part = nullptr;
+  p.splits = 1; p.parts = 1; p.dk_part = p.dv_part = nullptr;
   p.scale = d->scale;
   Buckets& t = p.bk;
   t.n = t.side = t.exact = t.nborders = t.reach = t.two_sided = 0;

@@ -15,7 +15,6 @@ using namespace tok;
 namespace {
 
 constexpr int CUS = 256;
-constexpr int STEP_BLOCKS = 1024;      // blocks that a step-form call is split into
 constexpr int SPLIT_KEYS = 512;        // fewest keys of a split where a call has more than 32 rows per key head
 
 // Scores of one wave's 32 queries against 32 NT keys, turned into probabilities in place (relative to 2^m, not normalised);
@@ -232,7 +231,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   const int qlo = start + (one ? rb * 32 % p.Sq : 0), qhi = start + (one ? r_last % p.Sq : p.Sq - 1);
   int kend = limit;
   if (p.causal) kend = min(kend, qhi + 1);
-  const int k_lo = split * p.chunk, k_hi = min(kend, k_lo + p.chunk);
+  // the splits share the keys that are there, not the cache's length
+  const int chunk = ((kend + p.splits - 1) / p.splits + 32 * WAVES - 1) / (32 * WAVES) * (32 * WAVES);
+  const int k_lo = split * chunk, k_hi = min(kend, k_lo + chunk);
   const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
   const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qi * p.qs;
@@ -467,7 +468,7 @@ template <typename T, int D, int MAPS> __global__ __launch_bounds__(256) void at
 
 struct Plan {
   bool step;
-  int splits, chunk, rblocks;
+  int splits, rblocks;
   size_t lds, part_bytes;
 };
 
@@ -484,12 +485,14 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   if (!r.step) return r;
   r.rblocks = (int)((rows + 31) / 32);
   const long long base = (long long)p.B * p.Hkv * r.rblocks, keys = rows <= 32 ? KEYS : SPLIT_KEYS, most = (p.Sk + keys - 1) / keys;
-  long long want = rows <= 32 ? (STEP_BLOCKS + base - 1) / base : CUS / base;      // many rows: joining costs more than a few idle CUs
+  // one round of blocks: as many as the CUs hold at once (bf16 at 128 columns: one each; 32 ragged caches of 4096 keys 52 us with
+  // 256 blocks, 57 with 512, 64 with 1024).  Many rows: joining costs more than a few idle CUs.
+  long long each = 160 * 1024 / r.lds, blocks = CUS * (each > 4 ? 4 : each);
+  long long want = rows <= 32 ? (blocks + base - 1) / base : CUS / base;
   if (want < 1) want = 1;
   if (want > most) want = most;
   if (want > MAX_SPLITS) want = MAX_SPLITS;
-  r.chunk = (int)(((p.Sk + want - 1) / want + KEYS - 1) / KEYS * KEYS);
-  r.splits = (p.Sk + r.chunk - 1) / r.chunk;
+  r.splits = (int)want;
   r.part_bytes = r.splits > 1 ? (size_t)base * r.splits * part_floats<D, MAPS>() * 4 : 0;
   return r;
 }
@@ -503,7 +506,6 @@ template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t w
     EOVAE_CHECK_ARG(r.part_bytes == 0 || (ws && ws_bytes >= r.part_bytes), "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, r.part_bytes);
     p.part = (float*)ws;
     p.splits = r.splits;
-    p.chunk = r.chunk;
     const size_t base = (size_t)p.B * p.Hkv;
     const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 64 * step_waves<T, D>(), r.lds, p, st, who);
     if (rc || r.splits == 1) return rc;
