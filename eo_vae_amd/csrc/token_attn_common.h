@@ -77,6 +77,12 @@ __device__ __forceinline__ f32x16 mma(const Frag<float>& a, const Frag<float>& b
 __device__ __forceinline__ float ldf(const void* p, size_t i, int is_f32) {
   return is_f32 ? ((const float*)p)[i] : (float)((const __bf16*)p)[i];
 }
+// a bias in units of log 2; a finite one stays finite (the type's lowest value is no -infinity: a query that sees nothing else
+// still has a softmax)
+__device__ __forceinline__ float bias_log2(const void* p, size_t i, int is_f32) {
+  const float v = ldf(p, i, is_f32);
+  return v == -INFINITY ? v : fmaxf(v * LOG2E, -3.4028234e38f);
+}
 
 // 16 bytes per lane from `src` to LDS at `to` + 16 * lane.  The compiler does not count it: wait_dma() does.
 __device__ __forceinline__ void load_lds16(const void* src, unsigned to) {
@@ -305,7 +311,7 @@ __device__ __forceinline__ int start_of(const Params& p, int b) {
 __device__ __forceinline__ void fill_bias(const Params& p, float* tab, int head, int tid, int nthreads) {
   const int span = p.bk.reach + PAD;
   for (int i = tid; i <= 2 * span; i += nthreads)
-    tab[i] = ldf(p.bias, (size_t)bucket_of(p.bk, i - span) * p.H + head, p.bias_f32) * LOG2E;
+    tab[i] = bias_log2(p.bias, (size_t)bucket_of(p.bk, i - span) * p.H + head, p.bias_f32);
 }
 static inline int bias_entries(const Buckets& b) { return b.n ? 2 * (b.reach + PAD) + 1 : 0; }
 

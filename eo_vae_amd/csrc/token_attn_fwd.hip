@@ -250,7 +250,7 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   float far_l = 0.f, far_r = 0.f;
   if (p.bk.n) {
     for (int i = tid; i <= 2 * reach; i += 64 * WAVES) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
-    for (int i = tid; i < p.bk.n * G; i += 64 * WAVES) tab[i] = ldf(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32) * LOG2E;
+    for (int i = tid; i < p.bk.n * G; i += 64 * WAVES) tab[i] = bias_log2(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32);
     __syncthreads();
     far_l = tab[ids[0] * G + g];
     far_r = tab[ids[2 * reach] * G + g];

@@ -553,7 +553,7 @@ int check(const eovae_token_norm* d, const char* who, int mode) {
   EOVAE_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
   EOVAE_CHECK_ARG(d->dtype == EOVAE_F32 || d->dtype == EOVAE_BF16, "%s: dtype %d (0 fp32, 1 bf16)", who, d->dtype);
   EOVAE_CHECK_ARG(d->param_dtype == EOVAE_F32 || d->param_dtype == EOVAE_BF16, "%s: param dtype %d (0 fp32, 1 bf16)", who, d->param_dtype);
-  EOVAE_CHECK_ARG(d->rows >= 1 && d->rows <= (1ll << 40) && d->channels >= 1 && d->channels <= 8192, "%s: %lld rows of %d channels (1 .. 8192)", who,
+  EOVAE_CHECK_ARG(d->rows >= 1 && d->rows <= (1ll << 38) && d->channels >= 1 && d->channels <= 8192, "%s: %lld rows of %d channels (1 .. 8192)", who,
                   d->rows, d->channels);
   EOVAE_CHECK_ARG(d->gates >= 0 && d->gates <= (1ll << 30) && (d->gates == 0 || d->rows % d->gates == 0), "%s: %lld gate rows for %lld rows", who, d->gates,
                   d->rows);

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 
 import torch
 
@@ -80,7 +81,7 @@ def _ptr(t):
 
 
 def _like(t):
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return t.new_empty(t.shape)
 
 
 class _on:
@@ -196,9 +197,9 @@ def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional
         side = n // 2 if two_sided else n
         if not (side >= 2 and n <= MAX_BUCKETS and not (two_sided and n % 2)):
             raise ValueError(f'{what}: {n} buckets; wants 2 .. {MAX_BUCKETS}, bidirectional an even number of at least 4')
-        if not (side // 2 < max_distance <= MAX_REACH):
+        if not (isinstance(max_distance, int) and side // 2 < max_distance <= MAX_REACH):
             raise ValueError(f'{what}: max_distance {max_distance}, wants {side // 2} < max_distance <= {MAX_REACH}')
-        borders = _borders(side, int(max_distance))[0]
+        borders = _borders(side, max_distance)[0]
         bias_table = bias_table.contiguous()
     if lam is not None:
         if not (lam.shape == (h,)):
@@ -217,14 +218,15 @@ def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional
         if t is not None:
             if not (torch.is_tensor(t) and t.dtype == torch.int32 and t.shape == (b,) and t.is_contiguous()):
                 raise ValueError(f'{what}: {n} wants a contiguous int32 tensor [{b}]' + (' or an int' if n == 'query_start' else ''))
+    scale = float(dim // maps) ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= 1e30:
+        raise ValueError(f'{what}: scale {scale}')
     _check_gpu(what, q, k, v, lam, bias_table, kv_len, query_start)
-    if scale is None:
-        scale = float(dim // maps) ** -0.5
     if q.numel() == 0 or sk == 0:      # nothing to attend to: zeros, tied to the inputs so that gradients are zeros too
         zero = v.sum() * 0 + (0 if lam is None else lam.sum() * 0) + (0 if bias_table is None else bias_table.sum() * 0) + k.sum() * 0
         return q * 0 + zero.to(q.dtype)
     args = (_rows16(q), _rows16(k), _rows16(v), bias_table, None if lam is None else lam.contiguous(), kv_len, query_start)
-    rest = (maps, two_sided, borders, bool(causal), float(scale), start)
+    rest = (maps, two_sided, borders, bool(causal), scale, start)
     if _tracked(q, k, v, bias_table, lam):
         return TokenAttentionFn.apply(*args, rest)
     return _attention_forward(*args, False, rest)[0]
@@ -239,7 +241,7 @@ def rel_pos_attention(q, k, v, bias_table=None, *, max_distance=128, bidirection
     bias_table [buckets, heads] (None: no bias): of a side's n buckets the first n // 2 hold one distance each, the others grow
     by equal ratios up to max_distance; bidirectional: half of the table for keys behind and at the query, half for keys
     ahead; otherwise keys ahead count as distance 0.
-    kv_len (int32 [batch]): keys at and behind it are not read.  causal: a query sees the keys up to its own position.
+    kv_len (int32 [batch], taken as 0 .. keys): keys at and behind it are not read.  causal: a query sees the keys up to its own position.
     query_start (int, or int32 [batch]): position of the first query among the keys; by default the queries are the last of
     the keys.  With kv_len it has to be given where positions count: 0 for a padded batch, kv_len - queries for a cache that
     the newest tokens have been written to.  A query that sees no key gives zeros and takes no gradient.
@@ -303,7 +305,9 @@ class GatedNormFn(torch.autograd.Function):
         dy = torch.zeros_like(h) if dy is None else dy.contiguous()
         dz = None if dz is None else dz.contiguous()
         dh, dx = _like(h), _like(x)
-        grads = [None if t is None else _like(t) for t in (w1, b1, w2, b2, gate)]
+        have = [t is not None for t in (w1, b1, w2, b2)]
+        rows = iter(w1.new_empty((sum(have), w1.shape[0])).unbind(0))          # one allocation for the [channels] gradients
+        grads = [next(rows) if t else None for t in have] + [None if gate is None else _like(gate)]
         with _on(h) as stream:
             d = _describe_norm(h, x, w1, b1, w2, b2, gate, stats, ctx.rest, None, None, dy, dz, dh, dx, grads)
             lib, ref = L.load(), C.byref(d)
@@ -350,8 +354,10 @@ def gated_norm_residual(h, x, post_weight, gate=None, pre_weight=None, *, post_b
             raise ValueError(f'{what}: gate is {gate.dtype}, the weights {post_weight.dtype}')
         if not (gate.dim() >= 1 and gate.shape[-1] == c and (gate.dim() == 1 or gate.dim() == h.dim()) and lead[:k] == tuple(h.shape[:k])):
             raise ValueError(f'{what}: gate {tuple(gate.shape)} for h {tuple(h.shape)}: [channels], or the shape of h with ones behind its leading axes')
-    if not (float(eps) > 0):
+    if not 0 < float(eps) < math.inf:
         raise ValueError(f'{what}: eps {eps}')
+    if not math.isfinite(residual_scale):
+        raise ValueError(f'{what}: residual_scale {residual_scale}')
     _check_gpu(what, h, x, post_weight, post_bias, pre_weight, pre_bias, gate)
     if h.numel() == 0:
         tie = sum(t.sum() * 0 for t in (post_weight, post_bias, pre_weight, pre_bias, gate) if t is not None)

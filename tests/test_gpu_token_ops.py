@@ -235,6 +235,57 @@ def test_bucket_tables(buckets, max_distance, two_sided):
     run_and_check(x, 1, max_distance, two_sided)
 
 
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps', [1, 2])
+def test_the_longest_reach_at_the_widest_heads(maps, dtype):
+    x = make(1, 140, 900, 2, 2, 128, dtype, maps, 128, seed=13)
+    run_and_check(x, maps, 1024, True, start=300)
+    x = make(1, 1, 900, 4, 1, 128, dtype, maps, 128, seed=13)
+    run_and_check(x, maps, 1024, False, True, kv_len=[870], start=869)
+
+
+def test_lengths_outside_the_cache_and_starts_far_away():
+    from eo_vae_amd import token_ops as T
+    x = make(4, 3, 70, 2, 1, 64, BF, 1, 32, seed=15)
+    t = lambda a: torch.tensor(a, dtype=torch.int32, device='cuda')                       # noqa: E731
+    clamped = T.rel_pos_attention(x['q'], x['k'], x['v'], x['bias'], kv_len=t([70, 70, 0, 0]), query_start=t([67] * 4))
+    assert torch.equal(T.rel_pos_attention(x['q'], x['k'], x['v'], x['bias'], kv_len=t([71, 2 ** 31 - 1, -1, -2 ** 31]), query_start=t([67] * 4)), clamped)
+    assert torch.equal(clamped[2:], torch.zeros_like(clamped[2:]))
+    # positions beyond any distance: the last buckets' constant, which a softmax does not see
+    plain = T.rel_pos_attention(x['q'], x['k'], x['v'])
+    for far in (2 ** 31 - 1, -2 ** 31, 2 ** 30, -2 ** 30):
+        got = T.rel_pos_attention(x['q'], x['k'], x['v'], x['bias'], query_start=t([far] * 4))
+        assert (got.float() - plain.float()).abs().max() <= 2.0 ** -7 * plain.float().abs().max()
+
+
+@pytest.mark.parametrize('low', [float('-inf'), -3.0e38])
+@pytest.mark.parametrize('sq,sk', [(1, 400), (150, 400), (300, 2100)])
+def test_buckets_that_shut_keys_out(low, sq, sk):
+    """A bias of -infinity, or of nearly the type's lowest value, for every key at and behind distance 64 leaves the others alone."""
+    from eo_vae_amd import token_ops as T
+    x = make(1, sq, sk, 2, 2, 64, FP, 1, 2, seed=16)
+    for n in ('q', 'k', 'v'):
+        x[n].requires_grad_(True)
+    shut = torch.tensor([[0.0, 0.0], [low, low]], device='cuda')
+    wide = torch.zeros(64, 2, device='cuda')
+    wide[32:] = low                                    # 64 buckets, one-sided: 32 distances of their own, then up to 33
+    out = T.rel_pos_attention(x['q'], x['k'], x['v'], wide, max_distance=33, bidirectional=False, causal=True)
+    rel = torch.arange(sk)[None] - (sk - sq + torch.arange(sq))[:, None]
+    seen = ((rel <= 0) & (rel > -32)).cuda()
+    q, k, v = (x[n].detach().double() for n in ('q', 'k', 'v'))
+    s = torch.einsum('bqhd,bkhd->bhqk', q, k) / 8
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    want = torch.einsum('bhqk,bkhd->bqhd', p, v)
+    assert (out.double() - want).abs().max() < 1e-4 * want.abs().max()
+    dk, dv = torch.autograd.grad(out, [x['k'], x['v']], x['do'])
+    assert torch.isfinite(dk).all() and torch.isfinite(dv).all()
+    hidden = ~seen.any(0)
+    assert dk[:, hidden].abs().max() <= 1e-30 if hidden.any() else True
+    # nothing but shut keys: -infinity leaves no key, the lowest value leaves the scores alone
+    only = T.rel_pos_attention(x['q'], x['k'], x['v'], shut, max_distance=2, bidirectional=False, causal=True, query_start=sk + 5)
+    assert torch.equal(only, torch.zeros_like(only)) if low == -math.inf else torch.isfinite(only).all() and only.abs().max() > 0
+
+
 def test_a_far_long_range_reaches_the_last_buckets():
     x = make(1, 300, 1500, 1, 1, 32, FP, 1, 32, seed=9)
     run_and_check(x, 1, 128, True, start=600)

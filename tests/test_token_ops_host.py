@@ -38,6 +38,9 @@ def test_bucket_borders_are_exact():
     (dict(bias_table=t(130, 4)), 'buckets'),
     (dict(bias_table=t(32, 4), max_distance=8), 'max_distance'),
     (dict(bias_table=t(32, 4), max_distance=1025), 'max_distance'),
+    (dict(bias_table=t(32, 4), max_distance=64.0), 'max_distance'),
+    (dict(scale=float('nan')), 'scale'),
+    (dict(scale=float('inf')), 'scale'),
     (dict(kv_len=torch.zeros(2, dtype=torch.int64)), 'kv_len'),
     (dict(kv_len=torch.zeros(3, dtype=torch.int32)), 'kv_len'),
     (dict(kv_len=torch.zeros(2, dtype=torch.int32), causal=True), 'needs query_start'),
@@ -77,6 +80,8 @@ def test_differential_attention_refuses(lam, text):
     (dict(gate=t(2, 1, 15)), 'gate'),
     (dict(gate=t(16, dtype=torch.bfloat16)), 'gate'),
     (dict(eps=0.0), 'eps'),
+    (dict(eps=float('nan')), 'eps'),
+    (dict(residual_scale=float('inf')), 'residual_scale'),
 ])
 def test_residual_step_refuses(kw, text):
     a = dict(h=t(2, 3, 16), x=t(2, 3, 16), post_weight=t(16))
