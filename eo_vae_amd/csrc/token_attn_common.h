@@ -56,7 +56,8 @@ struct Params {
   float *dk_part, *dv_part;                   // [parts] of dk and dv in fp32, where a block walks only a part of the queries
   float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain (+inf: nothing visible); delta likewise
   long long qb, qs, qh, kb, ks, kh, vb, vs, vh;   // element strides: batch, token, head
-  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, parts;
+  int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, parts, level;
+  int* tiles_before;                          // [B + 1], step form with `level`: key tiles of the sequences before each
   float scale;
   Buckets bk;
 };
@@ -135,9 +136,11 @@ template <typename T, int D, int R = tile_rows<T, D>()> struct Tile {
   static constexpr int PER32 = 32 * CH / 64;
   static __device__ __forceinline__ void dma32(const T* base, long long stride, int row0, int limit, const char* lds, int lane) {
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds);
+    int l = lane;
+    asm volatile("" : "+v"(l));
 #pragma unroll
     for (int i = 0; i < PER32; ++i) {
-      const int c = lane + 64 * i, row = c / CH, r = row0 + row;
+      const int c = l + 64 * i, row = c / CH, r = row0 + row;
       load_lds16((const char*)(base + (long long)(r < limit ? r : limit - 1) * stride) + (((c % CH) ^ swz(row)) << 4), to + 1024u * i);
     }
   }
@@ -363,7 +366,7 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   p.vb = d->v_strides[0]; p.vs = d->v_strides[1]; p.vh = d->v_strides[2];
   p.B = d->batch; p.Sq = d->sq; p.Sk = d->sk; p.H = d->heads; p.Hkv = d->kv_heads; p.start = d->start; p.causal = d->causal ? 1 : 0;
   p.bias_f32 = d->bias_dtype == EOVAE_F32; p.lam_f32 = d->lam_dtype == EOVAE_F32;
-  p.splits = 1; p.parts = 1; p.dk_part = p.dv_part = nullptr;
+  p.splits = 1; p.level = 0; p.tiles_before = nullptr; p.parts = 1; p.dk_part = p.dv_part = nullptr;
   p.scale = d->scale;
   Buckets& t = p.bk;
   t.n = t.side = t.exact = t.nborders = t.reach = t.two_sided = 0;

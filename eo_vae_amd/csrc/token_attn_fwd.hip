@@ -207,6 +207,15 @@ template <int D, int MAPS> constexpr int part_floats() { return MAPS * 32 * (D +
 // loads only, so no barrier stands between the waves until they meet at the end, and one tile is on its way while one is used.
 template <typename T, int D> constexpr int step_waves() { return sizeof(T) * D > 256 ? 2 : 4; }
 
+// runs over all sequences where the registers allow the loop
+template <typename T, int D, int MAPS> constexpr bool step_levels() { return !(sizeof(T) == 4 && D == 128 && MAPS == 2); }
+// key tiles of a sequence in a step-form call with `level`
+__device__ __forceinline__ int step_tiles(const Params& p, int b, int keys) {
+  int kend = key_limit(p, b);
+  if (p.causal) kend = min(kend, start_of(p, b) + p.Sq);
+  return kend > 0 ? (kend + keys - 1) / keys : 0;
+}
+
 template <typename T, int D, int MAPS>
 __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(const Params p) {
   using TK = Tile<T, D>;
@@ -214,13 +223,70 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   char* mine = lds + wave * 4 * T32;                           // two of (K, V)
+  constexpr int KEYS = 32 * WAVES, THREADS = 64 * WAVES;
+  const bool level = step_levels<T, D, MAPS>() && p.level;
   const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
-  int j = (int)blockIdx.x;
-  const int split = j % p.splits;
-  j /= p.splits;
-  const int rb = j % rblocks;
-  j /= rblocks;
-  const int hk = j % p.Hkv, b = j / p.Hkv;
+  // bias: bucket per distance (one byte) and the key head's columns of the table; two LDS reads per score near the query, the
+  // last buckets' values (one pair per query head, so per lane) everywhere else
+  unsigned char* ids = (unsigned char*)(lds + WAVES * 4 * T32);
+  const int reach = p.bk.reach;
+  float* tab = (float*)(ids + (p.bk.n ? ((2 * reach + 1 + 15) & ~15) : 0));
+  int* before = (int*)(tab + p.bk.n * G);
+  if (p.bk.n)
+    for (int i = tid; i <= 2 * reach; i += THREADS) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
+  // Lengths that differ (level): the key tiles of all sequences and key heads form one line, cut into equal runs, one to a block;
+  // a run ends one sequence's part and begins the next where it has to.  Otherwise a block has one split of one row block.
+  long long t = 0, t_end = 1;
+  if (level) {
+    if (wave == 0) {
+      int sum = 0;
+      for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int b = b0 + lane;
+        int n = b < p.B ? step_tiles(p, b, KEYS) : 0, inc = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int up = __shfl_up(inc, o, 64);
+          if (lane >= o) inc += up;
+        }
+        if (b < p.B) before[b] = sum + inc - n;
+        sum += __shfl(inc, 63, 64);
+      }
+      if (lane == 0) before[p.B] = sum;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = tid; i <= p.B; i += THREADS) p.tiles_before[i] = before[i];
+    const long long tiles_all = (long long)before[p.B] * p.Hkv;
+    const long long runs = min(tiles_all, (long long)gridDim.x);   // no run is empty: every slot that a key head's tiles span is written
+    if ((long long)blockIdx.x >= runs) return;
+    t = tiles_all * blockIdx.x / runs;
+    t_end = tiles_all * (blockIdx.x + 1) / runs;
+  }
+  for (; t < t_end;) {
+  int b, hk, rb = 0, k_lo, k_hi, tiles = 1;
+  size_t slot = blockIdx.x;
+  if (level) {
+    int lo = 0, hi = p.B;                                        // the sequence with before[b] Hkv <= t < before[b + 1] Hkv
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if ((long long)before[mid] * p.Hkv <= t) lo = mid;
+      else hi = mid;
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+    const int n = __builtin_amdgcn_readfirstlane(before[b + 1] - before[b]), in = (int)(t - (long long)before[b] * p.Hkv);
+    hk = __builtin_amdgcn_readfirstlane(in / n);
+    const int first = __builtin_amdgcn_readfirstlane(in % n);
+    tiles = (int)(t_end - t < n - first ? t_end - t : n - first);
+    k_lo = first * KEYS;
+    k_hi = (first + tiles) * KEYS;
+    slot += b * p.Hkv + hk;
+  } else {
+    int j = (int)blockIdx.x / p.splits;
+    rb = j % rblocks;
+    j /= rblocks;
+    hk = j % p.Hkv;
+    b = j / p.Hkv;
+  }
   const int row = rb * 32 + (lane & 31);
   const bool live = row < rows;
   const int g = live ? row / p.Sq : 0, qi = live ? row % p.Sq : 0, h = hk * G + g;
@@ -231,9 +297,12 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   const int qlo = start + (one ? rb * 32 % p.Sq : 0), qhi = start + (one ? r_last % p.Sq : p.Sq - 1);
   int kend = limit;
   if (p.causal) kend = min(kend, qhi + 1);
-  // the splits share the keys that are there, not the cache's length
-  const int chunk = ((kend + p.splits - 1) / p.splits + 32 * WAVES - 1) / (32 * WAVES) * (32 * WAVES);
-  const int k_lo = split * chunk, k_hi = min(kend, k_lo + chunk);
+  if (!level) {      // the splits share the keys that are there, not the cache's length
+    const int chunk = ((kend + p.splits - 1) / p.splits + KEYS - 1) / KEYS * KEYS;
+    k_lo = (int)blockIdx.x % p.splits * chunk;
+    k_hi = k_lo + chunk;
+  }
+  k_hi = min(kend, k_hi);
   const T* kb = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* vb = (const T*)p.v + b * p.vb + hk * p.vh;
   const T* qp = (const T*)p.q + b * p.qb + h * p.qh + (long long)qi * p.qs;
@@ -242,15 +311,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
     TK::dma32(kb, p.ks, k0, k_hi, mine, lane);
     TK::dma32(vb, p.vs, k0, k_hi, mine + T32, lane);
   }
-  // bias: bucket per distance (one byte) and the key head's columns of the table; two LDS reads per score near the query, the
-  // last buckets' values (one pair per query head, so per lane) everywhere else
-  unsigned char* ids = (unsigned char*)(lds + WAVES * 4 * T32);
-  const int reach = p.bk.reach;
-  float* tab = (float*)(ids + (p.bk.n ? ((2 * reach + 1 + 15) & ~15) : 0));
   float far_l = 0.f, far_r = 0.f;
   if (p.bk.n) {
-    for (int i = tid; i <= 2 * reach; i += 64 * WAVES) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
-    for (int i = tid; i < p.bk.n * G; i += 64 * WAVES) tab[i] = bias_log2(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32);
+    for (int i = tid; i < p.bk.n * G; i += THREADS) tab[i] = bias_log2(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32);
     __syncthreads();
     far_l = tab[ids[0] * G + g];
     far_r = tab[ids[2 * reach] * G + g];
@@ -355,7 +418,7 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   constexpr int MROW = D + 4;
   float* meet = (float*)lds;
   float* stat = meet + WAVES * 32 * MROW;
-  float* part = p.part + (size_t)blockIdx.x * part_floats<D, MAPS>();
+  float* part = p.part + slot * part_floats<D, MAPS>();
   constexpr int ITEMS = 32 * D / 4 / (64 * WAVES);             // 4-column pieces of the [32][D] tile per thread
   f32x4 first[ITEMS];
 #pragma unroll
@@ -417,10 +480,13 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
       store4((T*)p.out + o_at, sum[0], sum[1], sum[2], sum[3]);
     }
   }
+  t += tiles;
+  if (t < t_end) __syncthreads();                                  // the next run's tiles come where the sums lie
+  }
 }
 
 // joins the splits of a row: one block per (b, key head, row); thread = (4 columns, every RUNS-th split), runs joined in order
-constexpr int MAX_SPLITS = 256;
+constexpr int MAX_SPLITS = 1024;
 template <typename T, int D, int MAPS> __global__ __launch_bounds__(256) void attn_join_kernel(const Params p) {
   constexpr int LANES = D / 4, RUNS = 256 / LANES, PF = part_floats<D, MAPS>();
   __shared__ float wt[MAX_SPLITS], red[8];
@@ -428,25 +494,39 @@ template <typename T, int D, int MAPS> __global__ __launch_bounds__(256) void at
   const int G = p.H / p.Hkv, rows = G * p.Sq, rblocks = (rows + 31) / 32;
   const int row = (int)blockIdx.x % rows, bk = (int)blockIdx.x / rows, hk = bk % p.Hkv, b = bk / p.Hkv;
   const int tid = threadIdx.x, d = 4 * (tid % LANES), run = tid / LANES, g = row / p.Sq, qi = row % p.Sq, h = hk * G + g;
-  const float* part = p.part + ((size_t)bk * rblocks + row / 32) * p.splits * PF;
+  size_t first = ((size_t)bk * rblocks + row / 32) * p.splits;
+  int splits = p.splits;
+  if (p.level) {                 // the runs that touch this key head's tiles: tile x is in run ((x + 1) runs - 1) / tiles
+    const long long all = (long long)p.tiles_before[p.B] * p.Hkv, runs = min(all, (long long)p.level), n = p.tiles_before[b + 1] - p.tiles_before[b];
+    const long long x = (long long)p.tiles_before[b] * p.Hkv + hk * n;
+    const long long i0 = n ? ((x + 1) * runs - 1) / all : 0, i1 = n ? ((x + n) * runs - 1) / all : -1;
+    first = (size_t)(i0 + bk);
+    splits = (int)(i1 - i0 + 1);
+  }
+  const float* part = p.part + first * PF;
   f32x4 o[MAPS];
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) {
     const float* st = part + MAPS * 32 * D + (a * 32 + row % 32) * 2;
-    const bool has = tid < p.splits;
-    const float ms = has ? st[(size_t)tid * PF] : -INFINITY, ls = has ? st[(size_t)tid * PF + 1] : 0.f;
-    const float wm = wave_max(ms);
+    float ms = -INFINITY;
+    for (int s = tid; s < splits; s += 256) ms = fmaxf(ms, st[(size_t)s * PF]);
+    ms = wave_max(ms);
     __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = wm;
+    if ((tid & 63) == 0) red[tid >> 6] = ms;
     __syncthreads();
-    const float mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = mm == -INFINITY ? 0.f : mm, f = exp2_(ms - base);
-    if (has) wt[tid] = f;
-    const float ws = wave_sum(f * ls);
-    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ws;
+    const float mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = mm == -INFINITY ? 0.f : mm;
+    float ls = 0.f;
+    for (int s = tid; s < splits; s += 256) {
+      const float f = exp2_(st[(size_t)s * PF] - base);
+      wt[s] = f;
+      ls += f * st[(size_t)s * PF + 1];
+    }
+    ls = wave_sum(ls);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = ls;
     __syncthreads();
     const float l = (red[4] + red[5]) + (red[6] + red[7]);
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int s = run; s < p.splits; s += RUNS) sum += wt[s] * *(const f32x4*)(part + (size_t)s * PF + (a * 32 + row % 32) * D + d);
+    for (int s = run; s < splits; s += RUNS) sum += wt[s] * *(const f32x4*)(part + (size_t)s * PF + (a * 32 + row % 32) * D + d);
     *(f32x4*)(&sums[run][d]) = sum;
     __syncthreads();
     if (run == 0) {
@@ -466,10 +546,12 @@ template <typename T, int D, int MAPS> __global__ __launch_bounds__(256) void at
   store4((T*)p.out + at, o[0][0], o[0][1], o[0][2], o[0][3]);
 }
 
+constexpr int LEVEL_BATCH = 1024;      // sequences whose lengths a block adds up for itself
+
 struct Plan {
   bool step;
-  int splits, rblocks;
-  size_t lds, part_bytes;
+  int splits, rblocks, level;            // level: blocks that share the tiles of all sequences, or 0
+  size_t lds, part_bytes, before_bytes;
 };
 
 template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
@@ -493,6 +575,15 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   if (want > most) want = most;
   if (want > MAX_SPLITS) want = MAX_SPLITS;
   r.splits = (int)want;
+  // Lengths of their own for the sequences: equal runs over all of them (32 caches of 1024 .. 4096 keys: 53 us with two splits
+  // each, the longest cache twice the mean; XX us in runs).
+  if (step_levels<T, D, MAPS>() && p.kv_len && rows <= 32 && want > 1 && p.B <= LEVEL_BATCH && r.lds + 4 * (size_t)(p.B + 1) <= 160 * 1024) {
+    r.level = (int)(base * most < blocks ? base * most : blocks);
+    r.lds += 4 * (size_t)(p.B + 1);
+    r.before_bytes = (4 * (size_t)(p.B + 1) + 15) & ~(size_t)15;
+    r.part_bytes = ((size_t)r.level + base) * part_floats<D, MAPS>() * 4 + r.before_bytes;
+    return r;
+  }
   r.part_bytes = r.splits > 1 ? (size_t)base * r.splits * part_floats<D, MAPS>() * 4 : 0;
   return r;
 }
@@ -504,10 +595,12 @@ template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t w
   const Plan r = plan_of<T, D, MAPS>(p);
   if (r.step) {
     EOVAE_CHECK_ARG(r.part_bytes == 0 || (ws && ws_bytes >= r.part_bytes), "%s: workspace of %zu bytes, needs %zu", who, ws_bytes, r.part_bytes);
-    p.part = (float*)ws;
+    p.part = (float*)((char*)ws + r.before_bytes);
+    p.tiles_before = (int*)ws;
     p.splits = r.splits;
+    p.level = r.level;
     const size_t base = (size_t)p.B * p.Hkv;
-    const int rc = launch(attn_step_kernel<T, D, MAPS>, base * r.rblocks * r.splits, 64 * step_waves<T, D>(), r.lds, p, st, who);
+    const int rc = launch(attn_step_kernel<T, D, MAPS>, r.level ? (size_t)r.level : base * r.rblocks * r.splits, 64 * step_waves<T, D>(), r.lds, p, st, who);
     if (rc || r.splits == 1) return rc;
     return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, 256, 0, p, st, who);
   }
