@@ -89,6 +89,16 @@ __device__ __forceinline__ float bias_log2(const void* p, size_t i, int is_f32) 
 __device__ __forceinline__ void load_lds16(const void* src, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src) : "memory", "m0");
 }
+// a pointer that is the same in every lane, in scalar registers
+__device__ __forceinline__ const char* scalar(const void* p) {
+  const unsigned long long v = (unsigned long long)p;
+  return (const char*)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                       (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)v));
+}
+// the same from a wave-uniform address and 32 bits of the lane's own: no vector instruction per load
+__device__ __forceinline__ void load_lds16(const void* base, unsigned off, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
 // until at most N of the wave's newest loads are still on their way
 template <int N> __device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // the wave's LDS reads are done: what they read may be overwritten
@@ -120,10 +130,11 @@ template <typename T, int D, int R = tile_rows<T, D>()> struct Tile {
     const int row = t / CH, col = ((t % CH) ^ swz(row)) << 4;
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds +
                                                                        (unsigned)(tid & ~63) * 16u));
-    if (row0 + ROWS <= limit) {
-      const char* src = (const char*)(base + (long long)row0 * stride + (long long)row * stride) + col;
+    if (row0 + ROWS <= limit && stride < (1ll << 31) / (long long)(sizeof(T) * ROWS)) {
+      const char* src = scalar(base + (long long)row0 * stride);
+      const unsigned off = (unsigned)row * (unsigned)(stride * (long long)sizeof(T)) + (unsigned)col;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) load_lds16(src + (long long)i * (256 / CH) * stride * (long long)sizeof(T), to + 4096u * i);
+      for (int i = 0; i < PER; ++i) load_lds16(src + (long long)i * (256 / CH) * stride * (long long)sizeof(T), off, to + 4096u * i);
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -138,6 +149,19 @@ template <typename T, int D, int R = tile_rows<T, D>()> struct Tile {
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) const char*)lds);
     int l = lane;
     asm volatile("" : "+v"(l));
+    if (row0 + 32 <= limit && stride < (1ll << 31) / (long long)(sizeof(T) * 32)) {
+      // 64 / CH rows a load; the swizzle repeats after eight rows, so after PHASES loads
+      constexpr int STEP = 64 / CH, PHASES = STEP >= 8 ? 1 : 8 / STEP;
+      const unsigned line = (unsigned)(stride * (long long)sizeof(T));
+      const char* src = scalar(base + (long long)row0 * stride);
+#pragma unroll
+      for (int f = 0; f < PHASES; ++f) {
+        const unsigned off = (unsigned)(l / CH) * line + (unsigned)(((l % CH) ^ swz(l / CH + f * STEP)) << 4);
+#pragma unroll
+        for (int i = f; i < PER32; i += PHASES) load_lds16(src + (long long)i * STEP * line, off, to + 1024u * i);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PER32; ++i) {
       const int c = l + 64 * i, row = c / CH, r = row0 + row;
