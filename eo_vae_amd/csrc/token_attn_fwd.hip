@@ -89,10 +89,10 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
 }
 
 // One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
-// key0: position of the tile's first key; qpos: this lane's query position; limit: keys visible at all.
+// r0: first row of the tile in LDS, key0: its position; qpos: this lane's query position; limit: keys visible at all.
 template <typename T, int D, int W, int NT>
 __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
-                                          float& m, float& l, float c, int map, int key0, int limit, int qpos, int qlo, int qhi, const float* tab,
+                                          float& m, float& l, float c, int map, int r0, int key0, int limit, int qpos, int qlo, int qhi, const float* tab,
                                           int lane) {
   using TK = Tile<T, D>;
   f32x16 s[NT];
@@ -100,7 +100,7 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
   for (int t = 0; t < NT; ++t) {
     s[t] = zero16();
 #pragma unroll
-    for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
+    for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, r0 + 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
   }
   bool moved;
   const float a = softmax_tile<NT>(p, s, m, l, moved, c, key0, limit, qpos, qlo, qhi, tab, lane);
@@ -114,12 +114,12 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
       Frag<T> pf;
       to_frag(pf, s[t], 8 * u);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) acc[j] = mma(TK::frag_t(lv, 32 * t + 16 * u, 32 * j, lane), pf, acc[j]);
+      for (int j = 0; j < D / 32; ++j) acc[j] = mma(TK::frag_t(lv, r0 + 32 * t + 16 * u, 32 * j, lane), pf, acc[j]);
     }
 }
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : 1) void attn_rows_kernel(const Params p) {
   constexpr int W = D / MAPS;                 // width of one map's queries and keys
   constexpr int RB = 128 / MAPS;              // query rows of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -151,12 +151,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
   float m = -INFINITY, l = 0.f;
   Stream<T, D> kv(lds);
   if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
-  constexpr int ROWS = Tile<T, D>::ROWS;
+  constexpr int ROWS = Tile<T, D>::ROWS, NT = sizeof(T) == 2 && D <= 64 ? 1 : ROWS / 32;      // 32-key tiles of one softmax step
   for (int k0 = 0; k0 < kend; k0 += ROWS) {
     kv.arrive();
     if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, limit, tid);
-    if (!p.causal || k0 <= qhi)
-      tile_step<T, D, W, ROWS / 32>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, k0, limit, qpos, qlo, qhi, tab, lane);
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROWS; r0 += 32 * NT)
+      if (k0 + r0 < kend && (!p.causal || k0 + r0 <= qhi))
+        tile_step<T, D, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, limit, qpos, qlo, qhi, tab, lane);
   }
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
