@@ -90,11 +90,12 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
 
 // One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
 // r0: first row of the tile in LDS, key0: its position; qpos: this lane's query position; limit: keys visible at all.
-template <typename T, int D, int W, int NT>
+template <typename T, int D, int MAPS> constexpr int row_tile() { return sizeof(T) == 2 && D == 128 && MAPS == 2 ? 32 : tile_rows<T, D>(); }
+template <typename T, int D, int R, int W, int NT>
 __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
                                           float& m, float& l, float c, int map, int r0, int key0, int limit, int qpos, int qlo, int qhi, const float* tab,
                                           int lane) {
-  using TK = Tile<T, D>;
+  using TK = Tile<T, D, R>;
   f32x16 s[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -119,11 +120,11 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
 }
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : 1) void attn_rows_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 : 2) : 1) void attn_rows_kernel(const Params p) {
   constexpr int W = D / MAPS;                 // width of one map's queries and keys
   constexpr int RB = 128 / MAPS;              // query rows of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* tab = (float*)(lds + Stream<T, D>::BYTES);
+  float* tab = (float*)(lds + Stream<T, D, row_tile<T, D, MAPS>()>::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int map = MAPS == 2 ? wave >> 1 : 0, wrow = 32 * (MAPS == 2 ? (wave & 1) : wave);
   const int nbh = p.B * p.H, tiles = (p.Sq + RB - 1) / RB;
@@ -149,16 +150,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : 2) : 1) void a
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   float m = -INFINITY, l = 0.f;
-  Stream<T, D> kv(lds);
+  Stream<T, D, row_tile<T, D, MAPS>()> kv(lds);
   if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
-  constexpr int ROWS = Tile<T, D>::ROWS, NT = sizeof(T) == 2 && D <= 64 ? 1 : ROWS / 32;      // 32-key tiles of one softmax step
+  constexpr int ROWS = row_tile<T, D, MAPS>(), NT = sizeof(T) == 2 && D * 2 / MAPS <= 128 ? 1 : ROWS / 32;      // 32-key tiles of one softmax step
   for (int k0 = 0; k0 < kend; k0 += ROWS) {
     kv.arrive();
     if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, limit, tid);
 #pragma unroll 1
     for (int r0 = 0; r0 < ROWS; r0 += 32 * NT)
       if (k0 + r0 < kend && (!p.causal || k0 + r0 <= qhi))
-        tile_step<T, D, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, limit, qpos, qlo, qhi, tab, lane);
+        tile_step<T, D, ROWS, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, limit, qpos, qlo, qhi, tab, lane);
   }
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -611,7 +612,7 @@ template <typename T, int D, int MAPS> int run_fwd(Params& p, void* ws, size_t w
     return launch(attn_join_kernel<T, D, MAPS>, base * (p.H / p.Hkv) * p.Sq, 256, 0, p, st, who);
   }
   constexpr int RB = 128 / MAPS;
-  size_t lds = (size_t)Stream<T, D>::BYTES + 4 * (size_t)bias_entries(p.bk);
+  size_t lds = (size_t)Stream<T, D, row_tile<T, D, MAPS>()>::BYTES + 4 * (size_t)bias_entries(p.bk);
   if (MAPS == 2 && lds < (size_t)64 * (D + 4) * 4) lds = (size_t)64 * (D + 4) * 4;
   return launch(attn_rows_kernel<T, D, MAPS>, (size_t)((p.Sq + RB - 1) / RB) * p.B * p.H, 256, lds, p, st, who);
 }

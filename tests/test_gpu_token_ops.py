@@ -183,9 +183,22 @@ def test_attention_and_gradients(maps, d, dtype, shape):
 
 @pytest.mark.parametrize('dtype', [FP, BF])
 @pytest.mark.parametrize('maps,d', [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)])
+@pytest.mark.parametrize('shape', [
+    dict(b=64, sq=37, sk=75, h=4, hk=4, buckets=8, max_distance=20),
+    dict(b=32, sq=150, sk=150, h=4, hk=4, causal=True, two_sided=False, buckets=16, max_distance=30, kv_len=[150, 0, 1, 64] * 8, start=0),
+    dict(b=32, sq=131, sk=200, h=8, hk=2)])
+def test_calls_that_fill_the_chip(maps, d, dtype, shape):
+    """At least 256 blocks of 128 rows: the forms that smaller calls do not take."""
+    s = dict(shape)
+    x = make(s.pop('b'), s.pop('sq'), s.pop('sk'), s.pop('h'), s.pop('hk'), d, dtype, maps, s.pop('buckets', 0), seed=17)
+    run_and_check(x, maps, **s)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps,d', [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)])
 @pytest.mark.parametrize('b,sq,sk,h,hk,lens', [
     (3, 1, 700, 8, 2, [700, 1, 333]), (2, 2, 129, 4, 4, [2, 129]), (1, 1, 4000, 1, 1, [3999]), (2, 5, 260, 6, 1, [5, 257]),
-    (2, 1, 50, 32, 1, [50, 0])])
+    (2, 1, 50, 32, 1, [50, 0]), (70, 1, 300, 2, 2, [(37 * i) % 301 for i in range(70)]), (3, 4, 3000, 8, 1, [3000, 129, 2047])])
 def test_single_tokens_on_a_cache(maps, d, dtype, b, sq, sk, h, hk, lens):
     x = make(b, sq, sk, h, hk, d, dtype, maps, 32, seed=5)
     for i, n in enumerate(lens):            # nothing behind a sequence's length is read
