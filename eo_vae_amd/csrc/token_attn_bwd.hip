@@ -73,9 +73,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   const int tile = tiles - 1 - (int)blockIdx.x / nbh;
   int b, hk, h;
   split_bh(p, (int)blockIdx.x % nbh, b, hk, h);
-  const int row0 = tile * RB, wrow = SPLIT ? 0 : 32 * wave, limit = key_limit(p, b), start = start_of(p, b);
+  const int row0 = tile * RB, wrow = SPLIT ? 0 : 32 * wave, start = uniform(start_of(p, b));
   const int rlast = min(row0 + RB, p.Sq) - 1;
-  int kend = limit;
+  int kend = uniform(key_limit(p, b));
   if (p.causal) kend = min(kend, start + rlast + 1);
   const int qrow = row0 + wrow + (lane & 31);
   const bool live = qrow < p.Sq;
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   const auto work = [&](const auto& ka, const auto& va, int key0) __attribute__((always_inline)) {
     const int klast = key0 + 32 * NT - 1;
     if (p.causal && key0 > qhi) return;
-    const bool whole = klast < limit && (!p.causal || klast <= qlo);
+    const bool whole = klast < kend && (!p.causal || klast <= qlo);
     const float* tb = tab + (reach + PAD) + key0 - qpos + 4 * half;
     float far = 0.f;
     int side = 0;
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, near ? tb[32 * t + 8 * (r >> 2) + (r & 3)] : far);
         if (!whole) {
-          const int last = min(limit - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
+          const int last = min(kend - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -228,13 +228,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     }
   };
   if constexpr (SPLIT) {
-    for (int k0 = 32 * wave; k0 < kend; k0 += 128) work(InMemory{kb, p.ks, k0, limit, lane}, InMemory{vb, p.vs, k0, limit, lane}, k0);
+    for (int k0 = 32 * wave; k0 < kend; k0 += 128) work(InMemory{kb, p.ks, k0, kend, lane}, InMemory{vb, p.vs, k0, kend, lane}, k0);
   } else {
     Stream<T, D> kv(lds);
-    if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
+    if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
     for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
       kv.arrive();
-      if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, limit, tid);
+      if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, kend, tid);
 #pragma unroll 1
       for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
         if (k0 + 32 * t0 < kend) work(Staged<T, D>{kv.a(), 32 * t0, lane}, Staged<T, D>{kv.b(), 32 * t0, lane}, k0 + 32 * t0);
@@ -346,7 +346,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   float* tab = tab0 + (SPLIT && p.bk.n ? wave * (2 * (reach + PAD) + 1) : 0);
   const int share = (int)blockIdx.x % p.parts, block = (int)blockIdx.x / p.parts, j0 = block % n, kblock = block / n * KB, b = j0 / p.Hkv, hk = j0 % p.Hkv;
-  const int limit = key_limit(p, b), start = start_of(p, b);
+  const int start = uniform(start_of(p, b));
+  int limit = uniform(key_limit(p, b));
+  if (p.causal) limit = max(0, min(limit, start + p.Sq));         // keys behind the last query: seen by none, not read, no gradient
   const int klo = kblock + (SPLIT ? 0 : 32 * wave), krow = klo + (lane & 31), khi = klo + 31;
   const bool live = krow < limit;
   const T* kp = (const T*)p.k + b * p.kb + hk * p.kh + (long long)krow * p.ks;

@@ -334,6 +334,9 @@ __device__ __forceinline__ int start_of(const Params& p, int b) {
   return s < -(1 << 30) ? -(1 << 30) : (s > (1 << 30) ? (1 << 30) : s);
 }
 
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // head's bias by distance, log2 domain: tab[rel + reach + PAD], rel in [-reach - PAD, reach + PAD]
 __device__ __forceinline__ void fill_bias(const Params& p, float* tab, int head, int tid, int nthreads) {
   const int span = p.bk.reach + PAD;

@@ -131,9 +131,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
   const int tile = tiles - 1 - (int)blockIdx.x / nbh;      // causal: the longest rows first
   int b, hk, h;
   split_bh(p, (int)blockIdx.x % nbh, b, hk, h);
-  const int row0 = tile * RB, limit = key_limit(p, b), start = start_of(p, b);
+  const int row0 = tile * RB, start = uniform(start_of(p, b));
   const int rlast = min(row0 + RB, p.Sq) - 1;
-  int kend = limit;
+  int kend = uniform(key_limit(p, b));                                 // keys behind it are seen by no row of the block, and not read
   if (p.causal) kend = min(kend, start + rlast + 1);
   const int qrow = row0 + wrow + (lane & 31);
   const bool live = qrow < p.Sq;
@@ -151,15 +151,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   float m = -INFINITY, l = 0.f;
   Stream<T, D, row_tile<T, D, MAPS>()> kv(lds);
-  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, limit, tid);
+  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
   constexpr int ROWS = row_tile<T, D, MAPS>(), NT = sizeof(T) == 2 && D * 2 / MAPS <= 128 ? 1 : ROWS / 32;      // 32-key tiles of one softmax step
   for (int k0 = 0; k0 < kend; k0 += ROWS) {
     kv.arrive();
-    if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, limit, tid);
+    if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, kend, tid);
 #pragma unroll 1
     for (int r0 = 0; r0 < ROWS; r0 += 32 * NT)
       if (k0 + r0 < kend && (!p.causal || k0 + r0 <= qhi))
-        tile_step<T, D, ROWS, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, limit, qpos, qlo, qhi, tab, lane);
+        tile_step<T, D, ROWS, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, kend, qpos, qlo, qhi, tab, lane);
   }
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -297,13 +297,13 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   const int row = rb * 32 + (lane & 31);
   const bool live = row < rows;
   const int g = live ? row / p.Sq : 0, qi = live ? row % p.Sq : 0, h = hk * G + g;
-  const int limit = key_limit(p, b), start = start_of(p, b), qpos = start + qi;
+  const int limit = uniform(key_limit(p, b)), start = uniform(start_of(p, b)), qpos = start + qi;
   // positions of the block's first and last query (all of them where its rows reach into a second head)
   const int r_last = min(rows, rb * 32 + 32) - 1;
   const bool one = rb * 32 / p.Sq == r_last / p.Sq;
   const int qlo = start + (one ? rb * 32 % p.Sq : 0), qhi = start + (one ? r_last % p.Sq : p.Sq - 1);
   int kend = limit;
-  if (p.causal) kend = min(kend, qhi + 1);
+  if (p.causal) kend = max(0, min(kend, qhi + 1));
   if (!level) {      // the splits share the keys that are there, not the cache's length
     const int chunk = ((kend + p.splits - 1) / p.splits + KEYS - 1) / KEYS * KEYS;
     k_lo = (int)blockIdx.x % p.splits * chunk;
@@ -584,7 +584,7 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   r.splits = (int)want;
   // Lengths of their own for the sequences: equal runs over all of them (32 caches of 1024 .. 4096 keys: 52 us with two splits
   // each, where the longest cache sets the time; 50 us in runs).
-  if (step_levels<T, D, MAPS>() && p.kv_len && rows <= 32 && want > 1 && p.B <= LEVEL_BATCH && r.lds + 4 * (size_t)(p.B + 1) <= 160 * 1024) {
+  if (step_levels<T, D, MAPS>() && p.kv_len && rows <= 32 && want > 1 && base * most < (1ll << 30) && p.B <= LEVEL_BATCH && r.lds + 4 * (size_t)(p.B + 1) <= 160 * 1024) {
     r.level = (int)(base * most < blocks ? base * most : blocks);
     r.lds += 4 * (size_t)(p.B + 1);
     r.before_bytes = (4 * (size_t)(p.B + 1) + 15) & ~(size_t)15;

@@ -244,7 +244,9 @@ def rel_pos_attention(q, k, v, bias_table=None, *, max_distance=128, bidirection
     kv_len (int32 [batch], taken as 0 .. keys): keys at and behind it are not read.  causal: a query sees the keys up to its own position.
     query_start (int, or int32 [batch]): position of the first query among the keys; by default the queries are the last of
     the keys.  With kv_len it has to be given where positions count: 0 for a padded batch, kv_len - queries for a cache that
-    the newest tokens have been written to.  A query that sees no key gives zeros and takes no gradient.
+    the newest tokens have been written to.  A query that sees no key gives zeros and takes no gradient.  Keys that no query
+    sees are not read; a NaN or an infinity in the values of a key reaches the queries that see it, and with causal it may reach
+    up to 127 queries before them.
 
     Few queries per key head (at most 32, heads that share it included) run split over the keys, so single tokens against
     a long cache fill the chip; other calls walk the keys once per 128 queries.  The [queries, keys] map is never stored."""

@@ -207,6 +207,27 @@ def test_single_tokens_on_a_cache(maps, d, dtype, b, sq, sk, h, hk, lens):
     run_and_check_padded(x, maps, lens, [n - sq for n in lens])
 
 
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps,d', [(1, 64), (2, 128)])
+@pytest.mark.parametrize('b,h,sq,sk,start', [(1, 2, 40, 300, 20), (70, 4, 40, 100, 20), (1, 2, 2, 100, 50), (1, 1, 300, 400, -100)])
+def test_keys_ahead_of_every_query_are_not_read(b, h, sq, sk, start, maps, d, dtype):
+    x = make(b, sq, sk, h, h, d, dtype, maps, 8, seed=18)
+    last = start + sq
+    y = dict(x)
+    for n, bad in (('k', float('nan')), ('v', float('inf'))):
+        y[n] = x[n].clone()
+        y[n][:, last:] = bad
+    kw = dict(max_distance=20, bidirectional=False, causal=True, query_start=start)
+    got, want = [], []
+    for z, out in ((x, want), (y, got)):
+        leaves = [z[n].requires_grad_(True) for n in ('q', 'k', 'v', 'bias', 'lam') if z[n] is not None]
+        o = call(z, maps, **kw)
+        out += [o.detach(), *torch.autograd.grad(o, leaves, x['do'])]
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    assert torch.equal(got[2][:, last:], torch.zeros_like(got[2][:, last:])) and torch.equal(got[3][:, last:], torch.zeros_like(got[3][:, last:]))
+
+
 def run_and_check_padded(x, maps, lens, start):
     from copy import copy
     y = copy(x)
