@@ -413,6 +413,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
       else if (klo - qhi >= reach) offs = 3 * TILE;
       else near = true;
     }
+    // one wave per SIMD: the second products' operands are requested before the scores' long way through exp2 (4 x 8 x 2048 causal,
+    // training as a whole: 377 -> 358 us)
+    constexpr bool EARLY = sizeof(T) == 2 && D == 128 && MAPS == 2;
+    Frag<T> qt[EARLY ? 2 * D / 32 : 1], gt[EARLY ? 2 * D / 32 : 1];
     f32x16 da[NT], mix[MAPS == 2 ? NT : 1];
     const auto add_dv = [&](const f32x16 (&w)[NT]) __attribute__((always_inline)) {
 #pragma unroll
@@ -422,7 +426,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
           Frag<T> pf;
           to_frag(pf, w[t], 8 * u);
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) dv[j] = mma(ga.frag_t(32 * t + 16 * u, 32 * j), pf, dv[j]);
+          for (int j = 0; j < D / 32; ++j) dv[j] = mma(EARLY ? gt[EARLY ? u * (D / 32) + j : 0] : ga.frag_t(32 * t + 16 * u, 32 * j), pf, dv[j]);
         }
     };
 #pragma unroll
@@ -440,6 +444,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
         s[t] = zero16();
 #pragma unroll
         for (int i = 0; i < W / 16; ++i) s[t] = mma(qa.frag(32 * t, a * (W / 16) + i), kf[a * (W / 16) + i], s[t]);
+      }
+      if constexpr (EARLY) {
+        if (a == 0)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+              qt[u * (D / 32) + j] = qa.frag_t(16 * u, 32 * j);
+              gt[u * (D / 32) + j] = ga.frag_t(16 * u, 32 * j);
+            }
       }
       const float* ls = rows + a * 4 * TILE + 4 * half;
       float cc = c;
@@ -491,7 +505,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
           to_frag(sf, s[t], 8 * u);
 #pragma unroll
           for (int j = 0; j < W / 32; ++j)
-            dk[a * (W / 32) + j] = mma(qa.frag_t(32 * t + 16 * u, a * W + 32 * j), sf, dk[a * (W / 32) + j]);
+            dk[a * (W / 32) + j] = mma(EARLY ? qt[EARLY ? u * (D / 32) + a * (W / 32) + j : 0] : qa.frag_t(32 * t + 16 * u, a * W + 32 * j), sf, dk[a * (W / 32) + j]);
         }
     }
   };

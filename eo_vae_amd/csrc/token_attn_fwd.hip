@@ -6,7 +6,7 @@
 // map 1 of the same rows (same K / V tiles, half of K's columns each) and meet once at the end.  One wave reads 32 KiB of LDS
 // for 1024 cycles of matrix instructions at 128 columns, which is what the four waves' share of the LDS gives, and 32 exp2 at a
 // quarter of the vector rate beside them; two waves per SIMD overlap the three.  Measured: 16 heads x 8191 causal x 128
-// columns 308 us (893 TFLOP/s), 16 x 8 x 1024 x 64 55 us without a bias (630), two maps 16 x 8 x 1000 ragged 104 us.
+// columns 295 us (930 TFLOP/s), 16 x 8 x 1024 x 64 55 us without a bias (630), two maps 16 x 8 x 1000 ragged 105 us.
 // Step form (few rows per key head, e.g. single tokens against a cache, or a call too small to fill the chip): the rows are the
 // query heads that share one key head times the query tokens, 32 of them to a block, the four waves take different keys, the
 // key axis is also split over blocks where it is long, and then a second kernel joins the partial sums.  Bound by bytes where a
