@@ -602,6 +602,26 @@ def test_residual_step(lead, c, gate, layer, dtype):
 
 
 @pytest.mark.parametrize('layer', [False, True])
+def test_residual_step_gradients_against_differences(layer):
+    x = make_norm((3, 3), 40, FP, layer, (3, 1), seed=2)
+    y, z, grads = run_norm(x, layer, 0.75)
+    g = torch.Generator().manual_seed(1)
+    eps = 2.0 ** -7
+    for n, grad in grads.items():
+        step = torch.randn(x[n].shape, generator=g).cuda()
+        f = []
+        for sign in (1, -1):
+            t = {m: (None if a is None else a.detach().clone()) for m, a in x.items()}
+            t[n] = t[n] + sign * eps * step
+            y, z, _ = run_norm(t, layer, 0.75)
+            f.append((y.double() * x['dy'].double()).sum() + (z.double() * x['dz'].double()).sum())
+        slope, want = float((f[0] - f[1]).detach()) / (2 * eps), float((grad.double() * step.double()).sum())
+        # central difference: the next term is of the order of eps^2 (6e-5) of the slope's parts; 720 values off by some 2^-22 over 2 eps
+        size = float((grad.double() * step.double()).abs().sum())
+        assert abs(slope - want) < 2e-3 * size + 720 * 2.0 ** -22 / (2 * eps), (n, slope, want)
+
+
+@pytest.mark.parametrize('layer', [False, True])
 def test_residual_step_without_a_second_norm_and_with_fp32_weights(layer):
     x = make_norm((3, 50), 320, BF, layer, (3, 1), second=False, param=FP)
     y, z, grads = run_norm(x, layer)
