@@ -121,6 +121,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
       for (int i = lane; i < ntab; i += 64) diag[i] = 0.f;
       for (int i = lane; i < SCR_FLOATS; i += 64) scr[i] = 0.f;
     }
+    if constexpr (SPLIT) __syncthreads();      // the table is every thread's work; the streamed form's first barrier is its first tile's
   }
   f32x16 acc[D / 32];
 #pragma unroll

@@ -1,0 +1,24 @@
+"""Token operators (eo_vae_amd.token_ops) at their edges, against their definitions in 64 bits (bounds as in test_gpu_token_ops)."""
+import pytest
+import torch
+
+from test_gpu_token_ops import BF, FP, call, make, run_and_check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('maps,d', [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)])
+@pytest.mark.parametrize('b,sq,sk,h,hk,buckets,max_distance,two_sided,causal,start', [
+    (1, 141, 141, 4, 4, 32, 128, True, False, None),
+    (2, 577, 577, 4, 4, 32, 128, True, False, None),
+    (1, 70, 900, 2, 1, 128, 1024, True, False, 300),      # the widest table
+    (1, 40, 700, 2, 2, 8, 20, False, True, 650)])         # most tiles behind the last border: they read the table first of all
+def test_small_fp32_backward_repeats_its_bits(b, sq, sk, h, hk, buckets, max_distance, two_sided, causal, start, maps, d):
+    x = make(b, sq, sk, h, hk, d, FP, maps, buckets, seed=31)
+    out, grads = run_and_check(x, maps, max_distance, two_sided, causal, start=start)
+    leaves = [x[n] for n in ('q', 'k', 'v', 'bias', 'lam') if x[n] is not None]
+    for _ in range(4):
+        again = call(x, maps, max_distance=max_distance, bidirectional=two_sided, causal=causal, query_start=start)
+        assert torch.equal(again, out)
+        for a, e in zip(torch.autograd.grad(again, leaves, x['do']), grads):
+            assert torch.equal(a, e)

@@ -1,0 +1,43 @@
+"""CPU: what the token operators (eo_vae_amd.token_ops) keep, refuse and compile to."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+from eo_vae_amd import build as B
+
+
+def listing(name):
+    """The compiler's gfx950 output for one kernel source, as {kernel: [instruction, ...]}."""
+    hipcc = shutil.which('hipcc') or '/opt/rocm/bin/hipcc'
+    if not os.path.exists(hipcc):
+        pytest.skip('hipcc not available')
+    run = subprocess.run([hipcc, *B.NO_PACKED_FP32, f'--offload-arch={B.ARCH}', '-O3', '-std=c++17', '--offload-device-only', '-S',
+                          os.path.join(B.CSRC, name), '-o', '-'], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-2000:]
+    out, now = {}, None
+    for line in run.stdout.split('\n'):
+        m = re.match(r'(_Z\w+):', line)
+        if m:
+            now = out.setdefault(m.group(1), [])
+        elif line.startswith('.Lfunc_end'):
+            now = None
+        elif now is not None and line.startswith('\t') and line[1:2] not in '.;':
+            now.append(line.split()[0])
+    return out
+
+
+def test_the_shared_bias_table_is_complete_before_a_wave_reads_it():
+    """fp32 dQ of few rows reads keys from memory, so no tile's arrival stands between the block's filling of its bias table and
+    the first scores: a barrier of its own has to.  (Instructions up to the key loop's first product lie in program order.)"""
+    found = 0
+    for name, code in listing('token_attn_bwd.hip').items():
+        if 'attn_dq_kernelIf' not in name or 'ELb1E' not in name:
+            continue
+        found += 1
+        before = code[:next(i for i, op in enumerate(code) if op.startswith('v_mfma'))]
+        fill = max(i for i, op in enumerate(before) if op.startswith('ds_write'))
+        assert 's_barrier' in before[fill:], name
+    assert found == 5                                        # widths 32, 64, 128 of one map, 64, 128 of two
