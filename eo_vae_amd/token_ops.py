@@ -42,10 +42,10 @@ def bucket_borders(side, max_distance):
 
 @functools.lru_cache(maxsize=64)
 def _borders(side, max_distance):
-    """`bucket_borders` as the C array a descriptor points to; the cache keeps it alive."""
+    """`bucket_borders` as the C array a descriptor points to.  Whoever keeps its address for later (a backward) keeps the array:
+    the cache lets go of it."""
     edge = bucket_borders(side, max_distance)
-    arr = (C.c_int * max(1, len(edge)))(*edge)
-    return C.addressof(arr), arr
+    return (C.c_int * max(1, len(edge)))(*edge)
 
 
 def _check_gpu(what, t, *others):
@@ -123,9 +123,9 @@ def _describe(q, k, v, out, out2, lse, bias, lam, kv_len, query_start, rest, d_o
     b, sq, h, dim = q.shape
     return L.TokenAttention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out2), _ptr(lse), _ptr(d_out), _ptr(dq), _ptr(dk), _ptr(dv),
-        _ptr(dbias), _ptr(dlam), _ptr(bias), _ptr(lam), _ptr(kv_len), _ptr(query_start), borders, None, 0, q.stride()[:3], k.stride()[:3],
-        v.stride()[:3], _DTYPES[q.dtype], 0 if bias is None else _DTYPES[bias.dtype], 0 if lam is None else _DTYPES[lam.dtype], maps, b, sq,
-        k.shape[1], h, k.shape[2], dim, start, causal, 0 if bias is None else bias.shape[0], two_sided, scale)
+        _ptr(dbias), _ptr(dlam), _ptr(bias), _ptr(lam), _ptr(kv_len), _ptr(query_start), None if borders is None else C.addressof(borders), None, 0,
+        q.stride()[:3], k.stride()[:3], v.stride()[:3], _DTYPES[q.dtype], 0 if bias is None else _DTYPES[bias.dtype], 0 if lam is None else _DTYPES[lam.dtype], maps,
+        b, sq, k.shape[1], h, k.shape[2], dim, start, causal, 0 if bias is None else bias.shape[0], two_sided, scale)
 
 
 def _attention_forward(q, k, v, bias, lam, kv_len, query_start, keep, rest):
@@ -199,7 +199,7 @@ def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional
             raise ValueError(f'{what}: {n} buckets; wants 2 .. {MAX_BUCKETS}, bidirectional an even number of at least 4')
         if not (isinstance(max_distance, int) and side // 2 < max_distance <= MAX_REACH):
             raise ValueError(f'{what}: max_distance {max_distance}, wants {side // 2} < max_distance <= {MAX_REACH}')
-        borders = _borders(side, max_distance)[0]
+        borders = _borders(side, max_distance)
         bias_table = bias_table.contiguous()
     if lam is not None:
         if not (lam.shape == (h,)):

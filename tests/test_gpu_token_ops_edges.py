@@ -22,3 +22,16 @@ def test_small_fp32_backward_repeats_its_bits(b, sq, sk, h, hk, buckets, max_dis
         assert torch.equal(again, out)
         for a, e in zip(torch.autograd.grad(again, leaves, x['do']), grads):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+def test_other_bucket_tables_between_a_forward_and_its_backward(dtype):
+    x = make(1, 90, 150, 2, 2, 64, dtype, 1, 32, seed=32)
+    leaves = [x[n].requires_grad_(True) for n in ('q', 'k', 'v', 'bias')]
+    want = torch.autograd.grad(call(x, 1, max_distance=97), leaves, x['do'])
+    out = call(x, 1, max_distance=97)
+    with torch.no_grad():
+        for i in range(100):
+            call(x, 1, max_distance=100 + i)
+    for a, e in zip(torch.autograd.grad(out, leaves, x['do']), want):
+        assert torch.equal(a, e)

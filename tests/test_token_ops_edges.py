@@ -1,12 +1,16 @@
 """CPU: what the token operators (eo_vae_amd.token_ops) keep, refuse and compile to."""
+import ctypes as C
+import gc
 import os
 import re
 import shutil
 import subprocess
 
 import pytest
+import torch
 
 from eo_vae_amd import build as B
+from eo_vae_amd import token_ops as T
 
 
 def listing(name):
@@ -41,3 +45,21 @@ def test_the_shared_bias_table_is_complete_before_a_wave_reads_it():
         fill = max(i for i, op in enumerate(before) if op.startswith('ds_write'))
         assert 's_barrier' in before[fill:], name
     assert found == 5                                        # widths 32, 64, 128 of one map, 64, 128 of two
+
+
+def test_a_backward_still_has_its_borders_when_the_cache_has_let_go_of_them(monkeypatch):
+    kept = []
+    monkeypatch.setattr(T, '_check_gpu', lambda *a: None)
+    monkeypatch.setattr(T, '_attention_forward', lambda *a: kept.append(a) or (a[0], None, None))
+    q, bias = torch.zeros(1, 4, 2, 64), torch.zeros(32, 2)
+    T.rel_pos_attention(q, q, q, bias, max_distance=97)
+    *args, keep, rest = kept[0]
+    for i in range(100):
+        T.rel_pos_attention(q, q, q, bias, max_distance=100 + i)
+    kept.clear()
+    gc.collect()
+    other = [(C.c_int * 7)(*[-1] * 7) for _ in range(4096)]           # what a freed array's memory would be used for
+    q, k, v, bias, lam, kv_len, query_start = args
+    d = T._describe(q, k, v, q, None, None, bias, lam, kv_len, query_start, rest)
+    assert tuple((C.c_int * 7).from_address(d.borders)) == T.bucket_borders(16, 97)
+    assert other[0][0] == -1
