@@ -8,7 +8,8 @@ next to `ops.attention` and the generators' LayerNorm.
 
 float32 and bfloat16; statistics and sums are fp32 in either.  Every operator runs on the tensors' device and its current
 stream, allocates through torch (so calls of two streams or two captured graphs share nothing) and is differentiable;
-gradients are bit-reproducible.  Wrong arguments raise ValueError, tensors that are not on the GPU EovaeError."""
+gradients are bit-reproducible.  Forward-mode tangents and functional transforms are refused.  Wrong arguments raise ValueError,
+tensors that are not on the GPU EovaeError."""
 from __future__ import annotations
 
 import ctypes as C
@@ -16,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib as L
 
@@ -73,6 +75,10 @@ def _flat16(t):
 
 
 def _tracked(*tensors):
+    """Whether the call goes through its autograd function: a gradient may be asked for, or an input carries a forward-mode tangent
+    (which needs no grad mode, and which the function refuses rather than drops)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

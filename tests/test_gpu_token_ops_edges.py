@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from eo_vae_amd import token_ops as T
+
 from test_gpu_token_ops import BF, FP, call, make, run_and_check
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +37,20 @@ def test_other_bucket_tables_between_a_forward_and_its_backward(dtype):
             call(x, 1, max_distance=100 + i)
     for a, e in zip(torch.autograd.grad(out, leaves, x['do']), want):
         assert torch.equal(a, e)
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+    x = make(1, 20, 30, 2, 2, 64, FP, 2, 8, seed=33)
+    w = torch.ones(64, device='cuda')
+    with forward_ad.dual_level():
+        for n in ('q', 'k', 'v', 'bias', 'lam'):
+            y = dict(x)
+            y[n] = forward_ad.make_dual(x[n], torch.ones_like(x[n]))
+            with torch.no_grad(), pytest.raises(NotImplementedError, match='jvp'):
+                call(y, 2)
+        for n in range(3):
+            args = [x['q'], x['do'], w]
+            args[n] = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
+            with pytest.raises(NotImplementedError, match='jvp'):
+                T.gated_norm_residual(*args)

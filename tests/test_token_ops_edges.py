@@ -8,6 +8,7 @@ import subprocess
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from eo_vae_amd import build as B
 from eo_vae_amd import token_ops as T
@@ -63,3 +64,25 @@ def test_a_backward_still_has_its_borders_when_the_cache_has_let_go_of_them(monk
     d = T._describe(q, k, v, q, None, None, bias, lam, kv_len, query_start, rest)
     assert tuple((C.c_int * 7).from_address(d.borders)) == T.bucket_borders(16, 97)
     assert other[0][0] == -1
+
+
+@pytest.mark.parametrize('mode', ['grad mode', 'no grad mode', 'functional'])
+def test_forward_mode_tangents_are_refused(mode, monkeypatch):
+    monkeypatch.setattr(T, '_check_gpu', lambda *a: None)
+    monkeypatch.setattr(T, '_attention_forward', lambda q, *a: (q.clone(), None, None))
+    monkeypatch.setattr(T, '_norm_forward', lambda h, *a: (h.clone(), None, None))
+    q, lam, w = torch.randn(1, 4, 2, 64), torch.ones(2), torch.ones(64)
+    calls = {'q': lambda a: T.rel_pos_attention(a(q), q, q), 'v': lambda a: T.rel_pos_attention(q, q, a(q)),
+             'lam': lambda a: T.diff_attention(q, q, q, a(lam)), 'h': lambda a: T.gated_norm_residual(a(q), q, w)[0],
+             'weight': lambda a: T.gated_norm_residual(q, q, a(w))[0]}
+    for name, f in calls.items():
+        assert not f(lambda t: t).requires_grad
+        if mode == 'functional':
+            with pytest.raises(RuntimeError, match='functorch|data pointer'):
+                x = lam if name == 'lam' else w if name == 'weight' else q
+                torch.func.jvp(lambda t: f(lambda _: t), (x,), (x,))
+            continue
+        with forward_ad.dual_level(), torch.set_grad_enabled(mode == 'grad mode'), pytest.raises(NotImplementedError, match='jvp'):
+            f(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+    with forward_ad.dual_level():                             # nothing to refuse where no input has a tangent
+        assert torch.equal(calls['q'](lambda t: t), q)
