@@ -171,6 +171,20 @@ class TokenAttentionFn(torch.autograd.Function):
         return dq, dk, dv, dbias, dlam, None, None, None
 
 
+class NoKeysFn(torch.autograd.Function):
+    """Attention without keys (or queries): zeros and zero gradients whatever the inputs hold."""
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        ctx.like = [t if t is None else (t.shape, t.dtype, t.device) for t in inputs]
+        return inputs[0].new_zeros(inputs[0].shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        return tuple(torch.zeros(t[0], dtype=t[1], device=t[2]) if need else None for t, need in zip(ctx.like, ctx.needs_input_grad))
+
+
 def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional, causal, scale, kv_len, query_start):
     for n, t in (('q', q), ('k', k), ('v', v)):
         if not (t.dim() == 4):
@@ -228,9 +242,8 @@ def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional
     if not abs(scale) <= 1e30:
         raise ValueError(f'{what}: scale {scale}')
     _check_gpu(what, q, k, v, lam, bias_table, kv_len, query_start)
-    if q.numel() == 0 or sk == 0:      # nothing to attend to: zeros, tied to the inputs so that gradients are zeros too
-        zero = v.sum() * 0 + (0 if lam is None else lam.sum() * 0) + (0 if bias_table is None else bias_table.sum() * 0) + k.sum() * 0
-        return q * 0 + zero.to(q.dtype)
+    if q.numel() == 0 or sk == 0:      # nothing to attend to
+        return NoKeysFn.apply(q, k, v, bias_table, lam)
     args = (_rows16(q), _rows16(k), _rows16(v), bias_table, None if lam is None else lam.contiguous(), kv_len, query_start)
     rest = (maps, two_sided, borders, bool(causal), scale, start)
     if _tracked(q, k, v, bias_table, lam):

@@ -54,3 +54,22 @@ def test_forward_mode_tangents_are_refused():
             args[n] = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
             with pytest.raises(NotImplementedError, match='jvp'):
                 T.gated_norm_residual(*args)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps', [1, 2])
+def test_no_keys_at_all_as_with_lengths_of_zero(maps, dtype):
+    x = make(2, 3, 5, 2, 2, 64, dtype, maps, 8, seed=34)
+    x['bias'][2:] = float('-inf')
+    x['q'][0, 1] = float('inf')
+    none = torch.zeros(2, dtype=torch.int32, device='cuda')
+    want = call(x, maps, max_distance=20, kv_len=none, query_start=0)
+    empty = dict(x, k=x['k'][:, :0], v=x['v'][:, :0])
+    got = call(empty, maps, max_distance=20, query_start=0)
+    assert torch.equal(got, want) and torch.equal(got, torch.zeros_like(got))
+    leaves = [x[n].requires_grad_(True) for n in ('q', 'k', 'v', 'bias', 'lam') if x[n] is not None]
+    for keys in (5, 0):
+        y = dict(x, k=x['k'][:, :keys], v=x['v'][:, :keys])
+        out = call(y, maps, max_distance=20, kv_len=none, query_start=0)
+        for g in torch.autograd.grad(out, leaves, x['do']):
+            assert torch.equal(g, torch.zeros_like(g))

@@ -86,3 +86,27 @@ def test_forward_mode_tangents_are_refused(mode, monkeypatch):
             f(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
     with forward_ad.dual_level():                             # nothing to refuse where no input has a tangent
         assert torch.equal(calls['q'](lambda t: t), q)
+
+
+@pytest.mark.parametrize('maps', [1, 2])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_no_keys_give_zeros_whatever_the_inputs_hold(maps, dtype, monkeypatch):
+    monkeypatch.setattr(T, '_check_gpu', lambda *a: None)
+    q = torch.randn(2, 3, 2, 64).to(dtype)
+    q[0, 0], q[1, 2] = float('nan'), float('-inf')
+    k = torch.zeros(2, 0, 2, 64, dtype=dtype)
+    bias = torch.full((8, 2), float('-inf'))
+    lam = torch.tensor([float('inf'), 1.0])
+    leaves = [t.requires_grad_(True) for t in ((q, k, bias) if maps == 1 else (q, k, bias, lam))]
+    out = T.rel_pos_attention(q, k, k, bias) if maps == 1 else T.diff_attention(q, k, k, lam, bias)
+    assert out.dtype == dtype and torch.equal(out, torch.zeros_like(q)) and not torch.signbit(out).any()
+    for t, g in zip(leaves, torch.autograd.grad(out, leaves, torch.full_like(out, float('nan')))):
+        assert g.dtype == t.dtype and torch.equal(g, torch.zeros_like(t))
+    with torch.no_grad():
+        assert torch.equal(T.rel_pos_attention(q, k, k, bias), torch.zeros_like(q))
+    # no queries: zero gradients for the keys' side
+    keys = torch.full((2, 5, 2, 64), float('inf')).to(dtype).requires_grad_(True)
+    out = T.rel_pos_attention(q[:, :0], keys, keys, bias)
+    assert out.shape == (2, 0, 2, 64)
+    for t, g in zip((keys, bias), torch.autograd.grad(out, (keys, bias), torch.zeros_like(out))):
+        assert torch.equal(g, torch.zeros_like(t))
