@@ -20,6 +20,7 @@
 // dK/dV 97 (711 of four); 4 x 8 x 2048 x 128 dQ 121 us (850), dK/dV 174 (790); two maps of the same size 161 and 289.
 // No kernel here may spill: hipcc 7.2 has brought a value spilled half to registers, half to scratch back with a register missing.
 #include <math.h>
+#include <type_traits>
 #include "token_attn_common.h"
 
 using namespace tok;
@@ -115,8 +116,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     lse[a] = live ? p.lse[at] : INFINITY;
     if (live && half == 0 && (!SPLIT || wave == 0)) p.delta[at] = delta[a];
   }
+  float base = 0.f;
+  bool wide = false;
   if (p.bk.n) {
-    fill_bias(p, tab, h, tid, 256);
+    wide = wide_head(p, h, lane);
+    fill_bias(p, tab, h, tid, 256, wide);
+    if (wide) base = row_base(p, h, qpos, kend);
+    if (tid == 0 && b == 0 && tile == 0) p.wide[h] = wide;
+    if (wide && live && half == 0 && (!SPLIT || wave == 0)) p.base[((size_t)b * p.H + h) * p.Sq + qrow] = base;
     if (p.part) {
       for (int i = lane; i < ntab; i += 64) diag[i] = 0.f;
       for (int i = lane; i < SCR_FLOATS; i += 64) scr[i] = 0.f;
@@ -133,7 +140,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   for (int a = 0; a < MAPS; ++a) x[a] = m[a] = xl[a] = xr[a] = ml[a] = mr[a] = 0.f;
   const bool sums = p.part || p.lam_part;
   // 32 NT keys from position key0 on, their fragments from ka and va
-  const auto work = [&](const auto& ka, const auto& va, int key0) __attribute__((always_inline)) {
+  const auto work = [&](const auto& ka, const auto& va, int key0, auto wide_rows) __attribute__((always_inline)) {
+    constexpr bool WIDE_HEAD = decltype(wide_rows)::value;
     const int klast = key0 + 32 * NT - 1;
     if (p.causal && key0 > qhi) return;
     const bool whole = klast < kend && (!p.causal || klast <= qlo);
@@ -145,6 +153,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
       if (klast - qlo <= -reach) far = tab[PAD], side = -1;
       else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)], side = 1;
       else near = true;
+      if (WIDE_HEAD) far = 4.f * (far - base);
     }
     f32x16 da[NT];
 #pragma unroll
@@ -167,7 +176,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, near ? tb[32 * t + 8 * (r >> 2) + (r & 3)] : far);
+          for (int r = 0; r < 16; ++r) {
+            const int k = 32 * t + 8 * (r >> 2) + (r & 3);
+            if (WIDE_HEAD && r % 4 == 0) few_at_a_time();
+            s[t][r] = fmaf(s[t][r], c, near ? (WIDE_HEAD ? 4.f * (tb[k] - base) : tb[k]) : far);
+          }
         if (!whole) {
           const int last = min(kend - 1, p.causal ? qpos : 0x7fffffff) - key0 - 4 * half;     // last visible key
 #pragma unroll
@@ -228,19 +241,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
     }
   };
-  if constexpr (SPLIT) {
-    for (int k0 = 32 * wave; k0 < kend; k0 += 128) work(InMemory{kb, p.ks, k0, kend, lane}, InMemory{vb, p.vs, k0, kend, lane}, k0);
-  } else {
-    Stream<T, D> kv(lds);
-    if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
-    for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
-      kv.arrive();
-      if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, kend, tid);
+  const auto walk = [&](auto wide_rows) __attribute__((always_inline)) {
+    if constexpr (SPLIT) {
+      for (int k0 = 32 * wave; k0 < kend; k0 += 128) work(InMemory{kb, p.ks, k0, kend, lane}, InMemory{vb, p.vs, k0, kend, lane}, k0, wide_rows);
+    } else {
+      Stream<T, D> kv(lds);
+      if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
+      for (int k0 = 0; k0 < kend; k0 += TK::ROWS) {
+        kv.arrive();
+        if (k0 + TK::ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + TK::ROWS, kend, tid);
 #pragma unroll 1
-      for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
-        if (k0 + 32 * t0 < kend) work(Staged<T, D>{kv.a(), 32 * t0, lane}, Staged<T, D>{kv.b(), 32 * t0, lane}, k0 + 32 * t0);
+        for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
+          if (k0 + 32 * t0 < kend) work(Staged<T, D>{kv.a(), 32 * t0, lane}, Staged<T, D>{kv.b(), 32 * t0, lane}, k0 + 32 * t0, wide_rows);
+      }
     }
-  }
+  };
+  if (wide) walk(std::true_type{});        // a loop of its own: in one loop with the ordinary tiles it cost those 3 to 5 %
+  else walk(std::false_type{});
   if constexpr (SPLIT) {
     // the waves' sums over their keys: statistics into every wave, the output tile through the same LDS
     float* st = (float*)lds;
@@ -298,8 +315,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     const float* mid = d0 + reach + PAD;
     for (int u = tid; u < p.bk.n; u += 256) {
       const int right = p.bk.two_sided && u >= p.bk.side, i = right ? u - p.bk.side : u, last = p.bk.side - 1;
-      auto lo = [&](int n) { return n <= p.bk.exact ? n : p.bk.border[n - p.bk.exact - 1]; };
-      const int a = lo(i), z = i == last ? reach + PAD + 1 : lo(i + 1);    // distances a .. z - 1; behind them the far sums
+      const int a = first_distance(p.bk, i), z = i == last ? reach + PAD + 1 : first_distance(p.bk, i + 1);    // distances a .. z - 1; behind them the far sums
       float sum = 0.f;
 #pragma unroll 8
       for (int n = a; n < z; ++n) sum += right ? (n > 0 ? mid[n] : 0.f) : mid[-n];
@@ -329,8 +345,11 @@ template <typename T, int D, int MAPS> constexpr int dkv_head() {
   return v_in_lds<T, D, MAPS>() ? Stream<T, D, 32>::BYTES + Tile<T, D, 128>::BYTES : Stream<T, D>::BYTES;
 }
 
+// floats that dK/dV holds for a tile's rows
+template <int MAPS> constexpr int row_floats() { return (4 * MAPS + 1) * TILE; }
+
 template <typename T, int D, int MAPS, bool SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(256, D == 32 && !SPLIT ? 3 : sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) void attn_dkv_kernel(const Params p) {
   // bf16 at 128 columns, one map: two waves per SIMD leave 256 registers each, 160 of them accumulators and keys; the block's values stay in
   // LDS, and the stream's tiles are half as long, so that two blocks share a CU
   constexpr bool VLDS = v_in_lds<T, D, MAPS>();
@@ -339,10 +358,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   constexpr int W = D / MAPS;
   constexpr int NT = sizeof(T) == 2 && D * MAPS <= 64 ? 2 : 1, KB = SPLIT ? 32 : 128, STEP = SPLIT ? 32 : TK::ROWS;     // 32-query tiles worked on together, as the registers allow
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it); one set in use
-  // while the next is written, or one for each wave
+  // [MAPS][4][TILE]: delta, and -lse alone and with the bias of either last bucket (all a plain tile needs of it), then the rows'
+  // bases; one set in use while the next is written, or one for each wave
+  constexpr int ROWS = row_floats<MAPS>();
   float* rows2 = (float*)(lds + (SPLIT ? meet_bytes<D>() : (int)dkv_head<T, D, MAPS>()));
-  float* tab0 = rows2 + (SPLIT ? 4 : 2) * MAPS * 4 * TILE;
+  float* tab0 = rows2 + (SPLIT ? 4 : 2) * ROWS;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const int n = p.B * p.Hkv, G = p.H / p.Hkv, reach = p.bk.reach;
   float* tab = tab0 + (SPLIT && p.bk.n ? wave * (2 * (reach + PAD) + 1) : 0);
@@ -384,16 +404,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
         rd[a] = q0 + t < p.Sq ? p.delta[at] : 0.f;
       }
   };
-  const auto put_rows = [&](float* rows, int t) {
-    if (t < STEP)
+  const auto put_rows = [&](float* rows, int h, int q0, int t, auto wide_heads) {
+    if (t < STEP) {
+      float l = far_l, r = far_r;
+      if constexpr (decltype(wide_heads)::value) {
+        float base = 0.f;
+        if (p.wide[h]) base = q0 + t < p.Sq ? p.base[((size_t)b * p.H + h) * p.Sq + q0 + t] : 3.4e38f;         // behind the last row: above any entry
+        rows[MAPS * 4 * TILE + t] = base;
+        l = 4.f * (l - base);
+        r = 4.f * (r - base);
+      }
 #pragma unroll
       for (int a = 0; a < MAPS; ++a) {
         float* at = rows + a * 4 * TILE + t;
         at[0] = rd[a];
         at[TILE] = -rl[a];
-        at[2 * TILE] = far_l - rl[a];
-        at[3 * TILE] = far_r - rl[a];
+        at[2 * TILE] = l - rl[a];
+        at[3 * TILE] = r - rl[a];
+        if constexpr (decltype(wide_heads)::value)
+          if (rl[a] == INFINITY) at[2 * TILE] = at[3 * TILE] = -INFINITY;
       }
+    }
   };
   char* vlds = lds + Stream<T, D, TK::ROWS>::BYTES;
   const auto v_frag = [&](int i) __attribute__((always_inline)) {
@@ -402,7 +433,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
     else return frag_global(vp, i, lane, live);
   };
   // 32 NT queries from row r0 on, their fragments from qa and ga, their offsets at `rows`
-  const auto work = [&](const auto& qa, const auto& ga, const float* rows, int r0) __attribute__((always_inline)) {
+  const auto work = [&](const auto& qa, const auto& ga, const float* rows, int r0, auto wide_heads) __attribute__((always_inline)) {
+    constexpr bool WIDE_HEADS = decltype(wide_heads)::value;
     const int qlo = start + r0, qhi = qlo + 32 * NT - 1;
     if (r0 >= p.Sq || klo >= limit || (p.causal && qhi < klo)) return;
     const bool whole = khi < limit && (!p.causal || khi <= qlo);
@@ -459,10 +491,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
       const float* ls = rows + a * 4 * TILE + 4 * half;
       float cc = c;
       if (near) {
+        const float* bs = rows + MAPS * 4 * TILE + 4 * half;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], c, tb[-(32 * t + 8 * (r >> 2) + (r & 3))]);
+          for (int r = 0; r < 16; ++r) {
+            const int q = 32 * t + 8 * (r >> 2) + (r & 3);
+            if (WIDE_HEADS && r % 4 == 0) few_at_a_time();
+            s[t][r] = fmaf(s[t][r], c, WIDE_HEADS ? 4.f * (tb[-q] - bs[q]) : tb[-q]);
+          }
         cc = 1.f;
       }
       if (!whole) {       // first query that sees this key
@@ -512,59 +549,66 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && D * MAPS <= 128 ? 2 : 1) voi
   };
   const T* q_of = (const T*)p.q + b * p.qb;
   const T* g_of = (const T*)p.d_o + (size_t)b * p.Sq * p.H * D;
-  if constexpr (SPLIT) {
-    float* rows = rows2 + wave * MAPS * 4 * TILE;
-    int held = -1;
-    for (int it = wave; it < total; it += 4) {
-      const int h = hk * G + it / per, q0 = first + it % per * STEP;
-      fetch_rows(h, q0, lane);
-      if (h != held) {
-        held = h;
-        if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
-        if (p.bk.n) {
-          fill_bias(p, tab, h, lane, 64);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          far_l = tab[PAD];
-          far_r = tab[2 * (reach + PAD)];
+  const auto walk = [&](auto wide_heads, int tid, int lane) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(tid), "+v"(lane));   // nothing in common with the other kind's walk: what both would share costs the registers
+    if constexpr (SPLIT) {                      // that the products' operands are requested into (16 x 8 x 1024 x 64: 108 us, else 117)
+      float* rows = rows2 + wave * ROWS;
+      int held = -1;
+      for (int it = wave; it < total; it += 4) {
+        const int h = hk * G + it / per, q0 = first + it % per * STEP;
+        fetch_rows(h, q0, lane);
+        if (h != held) {
+          held = h;
+          if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+          if (p.bk.n) {
+            fill_bias(p, tab, h, lane, 64, wide_heads);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            far_l = tab[PAD];
+            far_r = tab[2 * (reach + PAD)];
+          }
         }
+        put_rows(rows, h, q0, lane, wide_heads);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        work(InMemory{q_of + h * p.qh, p.qs, q0, p.Sq, lane}, InMemory{g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, lane}, rows, q0, wide_heads);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
-      put_rows(rows, lane);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      work(InMemory{q_of + h * p.qh, p.qs, q0, p.Sq, lane}, InMemory{g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, lane}, rows, q0);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-  } else {
-    Stream<T, D, TK::ROWS> qg(lds);
-    const auto fetch = [&](int it) {
-      const int h = hk * G + it / per, q0 = first + it % per * STEP;
-      qg.next(q_of + h * p.qh, p.qs, g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, tid);
-      fetch_rows(h, q0, tid);
-    };
-    // this block's part of the (head, query tile) list
-    const int it0 = (int)((long long)total * share / p.parts), it1 = (int)((long long)total * (share + 1) / p.parts);
-    if (VLDS && it0 < it1) VT::dma((const T*)p.v + b * p.vb + hk * p.vh, p.vs, kblock, limit, vlds, tid);
-    if (it0 < it1) fetch(it0);
-    for (int it = it0; it < it1; ++it) {
-      const int h = hk * G + it / per, q0 = first + it % per * STEP;
-      float* rows = rows2 + (it & 1) * MAPS * 4 * TILE;          // written while other waves may still read the other one
-      if (it == it0 || it % per == 0) {                             // a head begins
-        if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
-        if (p.bk.n) {
-          __syncthreads();
-          fill_bias(p, tab, h, tid, 256);
-          __syncthreads();
-          far_l = tab[PAD];
-          far_r = tab[2 * (reach + PAD)];
+    } else {
+      Stream<T, D, TK::ROWS> qg(lds);
+      const auto fetch = [&](int it) {
+        const int h = hk * G + it / per, q0 = first + it % per * STEP;
+        qg.next(q_of + h * p.qh, p.qs, g_of + (size_t)h * D, (long long)p.H * D, q0, p.Sq, tid);
+        fetch_rows(h, q0, tid);
+      };
+      // this block's part of the (head, query tile) list
+      const int it0 = (int)((long long)total * share / p.parts), it1 = (int)((long long)total * (share + 1) / p.parts);
+      if (VLDS && it0 < it1) VT::dma((const T*)p.v + b * p.vb + hk * p.vh, p.vs, kblock, limit, vlds, tid);
+      if (it0 < it1) fetch(it0);
+      for (int it = it0; it < it1; ++it) {
+        const int h = hk * G + it / per, q0 = first + it % per * STEP;
+        float* rows = rows2 + (it & 1) * ROWS;          // written while other waves may still read the other one
+        if (it == it0 || it % per == 0) {                             // a head begins
+          if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
+          if (p.bk.n) {
+            __syncthreads();
+            fill_bias(p, tab, h, tid, 256, wide_heads);
+            __syncthreads();
+            far_l = tab[PAD];
+            far_r = tab[2 * (reach + PAD)];
+          }
         }
-      }
-      put_rows(rows, tid);
-      qg.arrive();
-      if (it + 1 < it1) fetch(it + 1);
+        put_rows(rows, h, q0, tid, wide_heads);
+        qg.arrive();
+        if (it + 1 < it1) fetch(it + 1);
 #pragma unroll 1
-      for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
-        work(Staged<T, D, TK::ROWS>{qg.a(), 32 * t0, lane}, Staged<T, D, TK::ROWS>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0);
+        for (int t0 = 0; t0 < TK::ROWS / 32; t0 += NT)
+          work(Staged<T, D, TK::ROWS>{qg.a(), 32 * t0, lane}, Staged<T, D, TK::ROWS>{qg.b(), 32 * t0, lane}, rows + 32 * t0, q0 + 32 * t0, wide_heads);
+      }
     }
-  }
+  };
+  bool wide = false;                                               // one of the key head's heads is
+  for (int g = 0; g < G && p.bk.n; ++g) wide = wide || uniform(p.wide[hk * G + g]);
+  if (wide) walk(std::true_type{}, tid, lane);
+  else walk(std::false_type{}, tid, lane);
   if constexpr (SPLIT) {
     const long long ld = (long long)p.Hkv * D;
     meet_sum<T, D>((float*)lds, dk, p.scale, (T*)p.dk + ((size_t)b * p.Sk * p.Hkv + hk) * D, ld, klo, p.Sk, wave, lane);
@@ -622,8 +666,9 @@ __global__ __launch_bounds__(64) void attn_fold_kernel(const float* part, const 
 }
 
 struct Sizes {
-  size_t delta, part, lam, dkv;      // floats; dkv: of each of dk's and dv's parts together
+  size_t delta, base, wide, part, lam, dkv;      // floats; dkv: of each of dk's and dv's parts together
   int slots, parts;
+  size_t floats() const { return delta + base + wide + part + lam + 2 * dkv; }
 };
 constexpr int CUS = 256;
 bool split_rows(const eovae_token_attention* d) {
@@ -637,6 +682,8 @@ Sizes sizes_of(const Params& p, const eovae_token_attention* d, bool dbias, bool
   const int maps = d->maps, rb = split_rows(d) ? 32 : 128;
   s.slots = p.B * ((p.Sq + rb - 1) / rb);
   s.delta = ((size_t)p.B * p.H * maps * p.Sq + 3) & ~(size_t)3;
+  s.base = p.bk.n ? ((size_t)p.B * p.H * p.Sq + 3) & ~(size_t)3 : 0;
+  s.wide = p.bk.n ? ((size_t)p.H + 3) & ~(size_t)3 : 0;
   s.part = dbias ? ((size_t)s.slots * p.H * p.bk.n + 3) & ~(size_t)3 : 0;
   s.lam = dlam ? ((size_t)s.slots * p.H + 3) & ~(size_t)3 : 0;
   // Few key heads and a long key axis leave CUs without a block (and, causal, one long row of blocks): the queries are cut into
@@ -653,19 +700,22 @@ Sizes sizes_of(const Params& p, const eovae_token_attention* d, bool dbias, bool
 template <typename T, int D, int MAPS> int run_bwd(Params& p, const eovae_token_attention* d, hipStream_t st) {
   const char* who = "token_attention_bwd";
   const Sizes s = sizes_of(p, d, d->dbias, d->dlam);
-  const size_t need = 4 * (s.delta + s.part + s.lam + 2 * s.dkv);
+  const size_t need = 4 * s.floats();
   EOVAE_CHECK_ARG(d->ws && d->ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", who, d->ws_bytes, need);
   p.delta = (float*)d->ws;
-  if (d->dbias) p.part = p.delta + s.delta;
-  if (d->dlam) p.lam_part = p.delta + s.delta + s.part;
+  p.base = p.delta + s.delta;
+  p.wide = (int*)(p.base + s.base);
+  float* rest = p.base + s.base + s.wide;
+  if (d->dbias) p.part = rest;
+  if (d->dlam) p.lam_part = rest + s.part;
   p.parts = s.parts;
   if (s.parts > 1) {
-    p.dk_part = p.delta + s.delta + s.part + s.lam;
+    p.dk_part = rest + s.part + s.lam;
     p.dv_part = p.dk_part + s.dkv;
   }
   const size_t tiles = (size_t)Stream<T, D>::BYTES, tab = 4 * (size_t)bias_entries(p.bk);
   const size_t sums = d->dbias ? 4 * tab + 16 + 4 * 4 * SCR_FLOATS : 0;
-  const size_t rows = 4 * MAPS * 4 * TILE;
+  const size_t rows = 4 * row_floats<MAPS>();
   int rc = EOVAE_OK;
   const auto dq = [&](auto kernel, int rb, size_t head) {
     return launch(kernel, (size_t)((p.Sq + rb - 1) / rb) * p.B * p.H, 256, head + tab + sums, p, st, who);
@@ -706,7 +756,7 @@ size_t eovae_token_attention_workspace(const eovae_token_attention* d, int backw
   if (make_params(d, p, "token_attention_workspace", 0)) return 0;
   if (!backward) return tok_fwd_workspace(d, p);
   const Sizes s = sizes_of(p, d, d->bias != nullptr, d->maps == 2);
-  return 4 * (s.delta + s.part + s.lam + 2 * s.dkv);
+  return 4 * s.floats();
 }
 int eovae_token_attention_bwd(const eovae_token_attention* d, void* stream) {
   Params p;

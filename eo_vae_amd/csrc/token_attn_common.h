@@ -54,7 +54,9 @@ struct Params {
   const void *bias, *lam;
   const int *kv_len, *q_start;
   float *dk_part, *dv_part;                   // [parts] of dk and dv in fp32, where a block walks only a part of the queries
-  float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain (+inf: nothing visible); delta likewise
+  float *lse, *delta, *part, *lam_part;      // lse: [B][H][maps][Sq], log2 domain, relative to the row's base (+inf: nothing visible); delta likewise
+  float* base;                                // backward, from dQ to dK/dV: [B][H][Sq], rows of wide heads
+  int* wide;                                  // [H]
   long long qb, qs, qh, kb, ks, kh, vb, vs, vh;   // element strides: batch, token, head
   int B, Sq, Sk, H, Hkv, start, causal, bias_f32, lam_f32, splits, parts, level;
   int* tiles_before;                          // [B + 1], step form with `level`: key tiles of the sequences before each
@@ -78,12 +80,13 @@ __device__ __forceinline__ f32x16 mma(const Frag<float>& a, const Frag<float>& b
 __device__ __forceinline__ float ldf(const void* p, size_t i, int is_f32) {
   return is_f32 ? ((const float*)p)[i] : (float)((const __bf16*)p)[i];
 }
-// a bias in units of log 2; a finite one stays finite (the type's lowest value is no -infinity: a query that sees nothing else
-// still has a softmax)
-__device__ __forceinline__ float bias_log2(const void* p, size_t i, int is_f32) {
-  const float v = ldf(p, i, is_f32);
-  return v == -INFINITY ? v : fmaxf(v * LOG2E, -3.4028234e38f);
-}
+// A finite bias beyond WIDE (the type's lowest value as a mask, say) would swallow the scores that it is added to, and the logarithm
+// of a row's sum beside it; yet a query that sees nothing else still has a softmax.  A head with such an entry is `wide`: its
+// rows are worked on relative to their `base`, the largest bias among the keys that the row sees (row_base; a softmax does not
+// see a constant), and its table is held in QUARTER units of log 2, so that no entry and no difference of two leaves fp32.
+// Other heads have base 0; they are walked by loops of their own and pay nothing per score.
+constexpr float WIDE = 88.f, QUARTER = 0.25f * LOG2E;        // 88: about 2^7 in units of log 2, where lse still resolves 2^-16
+__device__ __forceinline__ bool wide_entry(float v) { return fabsf(v) > WIDE && fabsf(v) < INFINITY; }
 
 // 16 bytes per lane from `src` to LDS at `to` + 16 * lane.  The compiler does not count it: wait_dma() does.
 __device__ __forceinline__ void load_lds16(const void* src, unsigned to) {
@@ -337,11 +340,43 @@ __device__ __forceinline__ int start_of(const Params& p, int b) {
 // a value that is the same in every lane, in a scalar register
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// head's bias by distance, log2 domain: tab[rel + reach + PAD], rel in [-reach - PAD, reach + PAD]
-__device__ __forceinline__ void fill_bias(const Params& p, float* tab, int head, int tid, int nthreads) {
+// head's bias by distance, log2 domain (wide: QUARTER units): tab[rel + reach + PAD], rel in [-reach - PAD, reach + PAD]
+__device__ __forceinline__ void fill_bias(const Params& p, float* tab, int head, int tid, int nthreads, bool wide) {
   const int span = p.bk.reach + PAD;
+  const float unit = wide ? QUARTER : LOG2E;
   for (int i = tid; i <= 2 * span; i += nthreads)
-    tab[i] = bias_log2(p.bias, (size_t)bucket_of(p.bk, i - span) * p.H + head, p.bias_f32);
+    tab[i] = unit * ldf(p.bias, (size_t)bucket_of(p.bk, i - span) * p.H + head, p.bias_f32);
+}
+// one head's column of the table has a wide entry; the same in every lane of a wave
+__device__ __forceinline__ bool wide_head(const Params& p, int head, int lane) {
+  bool any = false;
+  for (int u = lane; u < p.bk.n; u += 64) any = any || wide_entry(ldf(p.bias, (size_t)u * p.H + head, p.bias_f32));
+  return __any(any);
+}
+// wide heads are rare: few LDS reads in flight, so that their path costs the ordinary one no registers
+__device__ __forceinline__ void few_at_a_time() { asm volatile("" ::: "memory"); }
+// the first distance of a side's bucket i
+__device__ __forceinline__ int first_distance(const Buckets& t, int i) { return i <= t.exact ? i : t.border[i - t.exact - 1]; }
+// largest of value(bucket) over the keys 0 .. last that a query at position qpos sees; 0 where there is none, or it is not finite
+template <typename V> __device__ __forceinline__ float row_base(const Buckets& t, int qpos, int last, V value) {
+  const int r0 = -qpos, r1 = last - qpos;                          // their distances key - query
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int u = 0; u < t.n && last >= 0; ++u) {
+    const bool right = t.two_sided && u >= t.side;
+    const int i = right ? u - t.side : u, a = right && i == 0 ? 1 : first_distance(t, i);
+    const bool open = i == t.side - 1;                             // the last bucket has no end
+    const int z = open ? 0 : first_distance(t, i + 1) - 1;         // distances a .. z
+    if (!open && z < a) continue;
+    const bool ahead = !t.two_sided && i == 0 && r1 >= 0;          // one-sided: keys ahead count as distance 0
+    const bool seen = right ? r1 >= a && (open || r0 <= z) : (r0 <= -a && (r1 >= -a || open || r1 >= -z)) || ahead;
+    if (seen) top = fmaxf(top, value(u));
+  }
+  return fabsf(top) < INFINITY ? top : 0.f;
+}
+// the same from the table in memory, for a query of a wide head that sees keys below `kend`
+__device__ __forceinline__ float row_base(const Params& p, int head, int qpos, int kend) {
+  return row_base(p.bk, qpos, min(kend - 1, p.causal ? qpos : 0x7fffffff), [&](int u) { return QUARTER * ldf(p.bias, (size_t)u * p.H + head, p.bias_f32); });
 }
 static inline int bias_entries(const Buckets& b) { return b.n ? 2 * (b.reach + PAD) + 1 : 0; }
 
@@ -387,7 +422,7 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;
   p.bias = d->bias; p.lam = d->lam;
   p.kv_len = d->kv_len; p.q_start = d->query_start;
-  p.lse = d->lse; p.delta = nullptr; p.part = nullptr; p.lam_part = nullptr;
+  p.lse = d->lse; p.delta = nullptr; p.base = nullptr; p.wide = nullptr; p.part = nullptr; p.lam_part = nullptr;
   p.qb = d->q_strides[0]; p.qs = d->q_strides[1]; p.qh = d->q_strides[2];
   p.kb = d->k_strides[0]; p.ks = d->k_strides[1]; p.kh = d->k_strides[2];
   p.vb = d->v_strides[0]; p.vs = d->v_strides[1]; p.vh = d->v_strides[2];

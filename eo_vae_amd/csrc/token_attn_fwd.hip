@@ -12,6 +12,7 @@
 // key axis is also split over blocks where it is long, and then a second kernel joins the partial sums.  Bound by bytes where a
 // cache is long: 32 caches of 1024 .. 4096 keys x 4 key heads x 128, bf16, 37 us (4.6 TB/s; copies reach 4.9) and 4 for the join.
 #include <math.h>
+#include <type_traits>
 #include "token_attn_common.h"
 
 using namespace tok;
@@ -27,9 +28,9 @@ constexpr int SPLIT_KEYS = 512;        // fewest keys of a split where a call ha
 // fp32 sums hold easily and which saves rescaling the output tile for almost every key tile.
 // Plain tiles (all pairs visible, one bias value) cost one fma and one exp2 per score; the others add bias and mask first.
 constexpr float SLACK = 8.f;
-template <int NT>
+template <int NT, bool WIDE_HEAD>
 __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], float& m, float& l, bool& moved, float c, int key0, int limit,
-                                              int qpos, int qlo, int qhi, const float* tab, int lane) {
+                                              int qpos, int qlo, int qhi, const float* tab, float base, int lane) {
   const int half = lane >> 5, klast = key0 + 32 * NT - 1;
   const bool whole = klast < limit && (!p.causal || klast <= qlo);
   float far = 0.f;
@@ -39,6 +40,7 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
     if (klast - qlo <= -reach) far = tab[PAD];                              // every pair at or behind the last border
     else if (key0 - qhi >= reach) far = tab[2 * (reach + PAD)];
     else near = true;
+    if (WIDE_HEAD) far = 4.f * (far - base);
   }
   if (near || !whole) {
     const float* tb = tab + (p.bk.reach + PAD) + key0 - qpos + 4 * half;
@@ -47,7 +49,8 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int k = 32 * t + 8 * (r >> 2) + (r & 3);
-        s[t][r] = fmaf(s[t][r], c, near ? tb[k] : far);
+        if (WIDE_HEAD && r % 4 == 0) few_at_a_time();
+        s[t][r] = fmaf(s[t][r], c, near ? (WIDE_HEAD ? 4.f * (tb[k] - base) : tb[k]) : far);
       }
     if (!whole) {
       // last visible key of this lane's query, relative to its first score
@@ -91,10 +94,10 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
 // One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
 // r0: first row of the tile in LDS, key0: its position; qpos: this lane's query position; limit: keys visible at all.
 template <typename T, int D, int MAPS> constexpr int row_tile() { return sizeof(T) == 2 && D == 128 && MAPS == 2 ? 32 : tile_rows<T, D>(); }
-template <typename T, int D, int R, int W, int NT>
+template <typename T, int D, int R, int W, int NT, bool WIDE_HEAD>
 __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, const Frag<T> (&qf)[W / 16], f32x16 (&acc)[D / 32],
                                           float& m, float& l, float c, int map, int r0, int key0, int limit, int qpos, int qlo, int qhi, const float* tab,
-                                          int lane) {
+                                          float base, int lane) {
   using TK = Tile<T, D, R>;
   f32x16 s[NT];
 #pragma unroll
@@ -104,7 +107,7 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
     for (int i = 0; i < W / 16; ++i) s[t] = mma(TK::frag(lk, r0 + 32 * t, map * (W / 16) + i, lane), qf[i], s[t]);
   }
   bool moved;
-  const float a = softmax_tile<NT>(p, s, m, l, moved, c, key0, limit, qpos, qlo, qhi, tab, lane);
+  const float a = softmax_tile<NT, WIDE_HEAD>(p, s, m, l, moved, c, key0, limit, qpos, qlo, qhi, tab, base, lane);
   if (moved)
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) acc[j] *= a;
@@ -120,7 +123,7 @@ __device__ __forceinline__ void tile_step(const Params& p, char* lk, char* lv, c
 }
 
 template <typename T, int D, int MAPS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 : 2) : 1) void attn_rows_kernel(const Params p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 : 2) : D == 32 ? 3 : 1) void attn_rows_kernel(const Params p) {
   constexpr int W = D / MAPS;                 // width of one map's queries and keys
   constexpr int RB = 128 / MAPS;              // query rows of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -145,22 +148,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
 #pragma unroll
   for (int i = 0; i < W / 16; ++i) qf[i] = frag_global(qp, i, lane, live);
   const float c = positive_scale(p.scale, qf);
-  if (p.bk.n) fill_bias(p, tab, h, tid, 256);
+  float base = 0.f;
+  bool wide = false;
+  if (p.bk.n) {
+    wide = wide_head(p, h, lane);
+    fill_bias(p, tab, h, tid, 256, wide);
+    if (wide) base = row_base(p, h, qpos, kend);
+  }
   f32x16 acc[D / 32];
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   float m = -INFINITY, l = 0.f;
-  Stream<T, D, row_tile<T, D, MAPS>()> kv(lds);
-  if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
   constexpr int ROWS = row_tile<T, D, MAPS>(), NT = sizeof(T) == 2 && D * 2 / MAPS <= 128 ? 1 : ROWS / 32;      // 32-key tiles of one softmax step
-  for (int k0 = 0; k0 < kend; k0 += ROWS) {
-    kv.arrive();
-    if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, kend, tid);
+  const auto walk = [&](auto wide_rows) __attribute__((always_inline)) {
+    Stream<T, D, ROWS> kv(lds);
+    if (kend > 0) kv.next(kb, p.ks, vb, p.vs, 0, kend, tid);
+    for (int k0 = 0; k0 < kend; k0 += ROWS) {
+      kv.arrive();
+      if (k0 + ROWS < kend) kv.next(kb, p.ks, vb, p.vs, k0 + ROWS, kend, tid);
 #pragma unroll 1
-    for (int r0 = 0; r0 < ROWS; r0 += 32 * NT)
-      if (k0 + r0 < kend && (!p.causal || k0 + r0 <= qhi))
-        tile_step<T, D, ROWS, W, NT>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, kend, qpos, qlo, qhi, tab, lane);
-  }
+      for (int r0 = 0; r0 < ROWS; r0 += 32 * NT)
+        if (k0 + r0 < kend && (!p.causal || k0 + r0 <= qhi))
+          tile_step<T, D, ROWS, W, NT, decltype(wide_rows)::value>(p, kv.a(), kv.b(), qf, acc, m, l, c, map, r0, k0 + r0, kend, qpos, qlo, qhi, tab, base,
+                                                                   lane);
+    }
+  };
+  if (wide) walk(std::true_type{});        // a loop of its own: the ordinary one pays nothing for it
+  else walk(std::false_type{});
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
@@ -238,7 +252,8 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
   unsigned char* ids = (unsigned char*)(lds + WAVES * 4 * T32);
   const int reach = p.bk.reach;
   float* tab = (float*)(ids + (p.bk.n ? ((2 * reach + 1 + 15) & ~15) : 0));
-  int* before = (int*)(tab + p.bk.n * G);
+  int* wides = (int*)(tab + p.bk.n * G);                       // [WAVES]: a wave has filled in a wide entry
+  int* before = wides + WAVES;
   if (p.bk.n)
     for (int i = tid; i <= 2 * reach; i += THREADS) ids[i] = (unsigned char)bucket_of(p.bk, i - reach);
   // Lengths that differ (level): the key tiles of all sequences and key heads form one line, cut into equal runs, one to a block;
@@ -318,12 +333,27 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
     TK::dma32(kb, p.ks, k0, k_hi, mine, lane);
     TK::dma32(vb, p.vs, k0, k_hi, mine + T32, lane);
   }
-  float far_l = 0.f, far_r = 0.f;
+  float far_l = 0.f, far_r = 0.f, base = 0.f;
   if (p.bk.n) {
-    for (int i = tid; i < p.bk.n * G; i += THREADS) tab[i] = bias_log2(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32);
+    bool any = false;
+    for (int i = tid; i < p.bk.n * G; i += THREADS) {
+      const float v = ldf(p.bias, (size_t)(i / G) * p.H + hk * G + i % G, p.bias_f32);
+      any = any || wide_entry(v);
+      tab[i] = QUARTER * v;                                        // here always in this unit: a few tiles look entries up
+    }
+    const bool mine_any = __any(any);
+    if (lane == 0) wides[wave] = mine_any;
     __syncthreads();
-    far_l = tab[ids[0] * G + g];
-    far_r = tab[ids[2 * reach] * G + g];
+    any = false;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any = any || wides[w];
+    if (any) {                                                     // only the lanes of the heads that are wide (as wide_head has it)
+      bool head = false;
+      for (int u = 0; u < p.bk.n; ++u) head = head || wide_entry(ldf(p.bias, (size_t)u * p.H + h, p.bias_f32));
+      if (head) base = row_base(p.bk, qpos, min(limit - 1, p.causal ? qpos : 0x7fffffff), [&](int u) { return tab[u * G + g]; });
+    }
+    far_l = 4.f * (tab[ids[0] * G + g] - base);
+    far_r = 4.f * (tab[ids[2 * reach] * G + g] - base);
   }
   Frag<T> qf[D / 16];
 #pragma unroll
@@ -370,7 +400,7 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
         if (near) {
           int rel = k0 + 4 * half + k - qpos;
           rel = rel < -reach ? -reach : (rel > reach ? reach : rel);
-          add = tab[ids[rel + reach] * G + g];
+          add = 4.f * (tab[ids[rel + reach] * G + g] - base);
         }
 #pragma unroll
         for (int a = 0; a < MAPS; ++a) s[a][r] = k > last ? -INFINITY : fmaf(s[a][r], c, add);
@@ -567,7 +597,7 @@ template <typename T, int D, int MAPS> Plan plan_of(const Params& p) {
   const long long G = p.H / p.Hkv, rows = G * p.Sq;
   const size_t bias = p.bk.n ? (size_t)((2 * p.bk.reach + 16) & ~15) + 4 * (size_t)p.bk.n * G : 0;
   const size_t meet = (size_t)WAVES * 32 * (D + 4) * 4 + WAVES * 32 * 2 * 4;
-  r.lds = WAVES * 4 * 32 * (size_t)Tile<T, D>::ROWB + bias;
+  r.lds = WAVES * 4 * 32 * (size_t)Tile<T, D>::ROWB + bias + 4 * WAVES;
   if (r.lds < meet) r.lds = meet;
   // Step form: few rows per key head (then only the key axis can fill the chip), or fewer blocks of the row form than CUs
   r.step = (rows <= 32 || (long long)p.B * p.H * ((p.Sq * (long long)MAPS + 127) / 128) < CUS) && r.lds <= 160 * 1024;

@@ -259,7 +259,8 @@ def rel_pos_attention(q, k, v, bias_table=None, *, max_distance=128, bidirection
     multiple of the key heads (head h reads key head h // (heads // key heads)).  scale: width^-0.5.
     bias_table [buckets, heads] (None: no bias): of a side's n buckets the first n // 2 hold one distance each, the others grow
     by equal ratios up to max_distance; bidirectional: half of the table for keys behind and at the query, half for keys
-    ahead; otherwise keys ahead count as distance 0.
+    ahead; otherwise keys ahead count as distance 0.  A bias of -infinity shuts keys out; a finite one never does (a query whose
+    keys all carry the type's lowest value has the softmax of its scores).
     kv_len (int32 [batch], taken as 0 .. keys): keys at and behind it are not read.  causal: a query sees the keys up to its own position.
     query_start (int, or int32 [batch]): position of the first query among the keys; by default the queries are the last of
     the keys.  With kv_len it has to be given where positions count: 0 for a padded batch, kv_len - queries for a cache that

@@ -503,7 +503,10 @@ int eovae_area_rot(const float* src, float* dst, int planes, int Hs, int Ws, int
  * bias [buckets][heads] (NULL: none).  One side has n = buckets (two_sided: buckets / 2) of them: distance d < n / 2 is
  * bucket d, then borders[i] (host memory, n - n / 2 - 1 ascending distances) is the first distance of bucket n / 2 + 1 + i;
  * two_sided: keys ahead of the query use the second half of the table, else they count as distance 0.
- * lse [batch][heads][maps][sq] (forward: nullable; the backward needs it), out2: the second map's own output (maps = 2; needed
+ * A finite bias of any size is a bias: a query whose keys all carry the type's lowest value has the softmax of its scores; -infinity
+ * shuts a key out.
+ * lse [batch][heads][maps][sq] (forward: nullable; the backward needs it, and both leave out a constant of the row where the table
+ * holds finite values beyond 88), out2: the second map's own output (maps = 2; needed
  * by the backward).  dbias [buckets][heads] and dlam [heads] are nullable and have the type of bias / lam.
  * ws: eovae_token_attention_workspace(d, backward) bytes (d as for the call, ws aside); 0 where none is needed or the
  * descriptor is refused.

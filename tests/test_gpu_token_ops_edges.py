@@ -4,7 +4,7 @@ import torch
 
 from eo_vae_amd import token_ops as T
 
-from test_gpu_token_ops import BF, FP, call, make, run_and_check
+from test_gpu_token_ops import BF, FP, call, inside, make, reference, run_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,86 @@ def test_no_keys_at_all_as_with_lengths_of_zero(maps, dtype):
         out = call(y, maps, max_distance=20, kv_len=none, query_start=0)
         for g in torch.autograd.grad(out, leaves, x['do']):
             assert torch.equal(g, torch.zeros_like(g))
+
+
+# A query whose visible keys all carry one very low (or high) finite bias has the softmax of its bare scores: the definition does not
+# change when a constant is added to all biases of a row.  So a table with an entry of -1e9 has to act as one whose entry lies
+# 200 below the others (e^-200 is 0 beside them, and 64 bits hold scores next to it).
+LEVELS = [(m, d, -1e9, -200.0) for m, d in [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)]] \
+    + [(m, d, a, e) for m, d in [(1, 64), (2, 128)] for a, e in [(-100.0, -100.0), (-3.0e38, -200.0), (torch.finfo(FP).min, -200.0), (3.0e38, 200.0)]]
+
+
+def level_check(x, maps, table, equal, max_distance, two_sided, causal=False, kv_len=None, start=None, scale=None):
+    x = dict(x, bias=table.to(x['q'].device))
+    leaves = {n: x[n].requires_grad_(True) for n in ('q', 'k', 'v', 'bias', 'lam') if x[n] is not None}
+    dev = lambda t: t if t is None or isinstance(t, int) else torch.tensor(t, dtype=torch.int32, device='cuda')   # noqa: E731
+    kw = dict(max_distance=max_distance, bidirectional=two_sided, causal=causal, kv_len=dev(kv_len), query_start=dev(start), scale=scale)
+    out = call(x, maps, **kw)
+    with torch.no_grad():
+        assert torch.equal(out, call(x, maps, **kw))
+    grads = torch.autograd.grad(out, list(leaves.values()), x['do'])
+    w = x['q'].shape[-1] // maps
+    val, err = reference(x['q'], x['k'], x['v'], x['do'], maps, w ** -0.5 if scale is None else scale, equal, x['lam'], max_distance, two_sided,
+                         causal, kv_len, start)
+    inside(out, val['out'], err['out'], 'out')
+    for n, g in zip(leaves, grads):
+        inside(g, val['d' + n], err['d' + n], 'd' + n)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('shape', [
+    dict(b=1, sq=70, sk=90, h=4, hk=2, two_sided=True),                                            # few blocks: step form, split backward
+    dict(b=64, sq=37, sk=75, h=4, hk=4, two_sided=True),                                           # the chip full: row form
+    dict(b=1, sq=90, sk=400, h=2, hk=1, two_sided=False, causal=True, start=330),                  # tiles of one bias value, causal
+    dict(b=40, sq=131, sk=300, h=4, hk=2, two_sided=False, causal=True, start=250, kv_len=[300, 40, 0, 129] * 10),
+    dict(b=3, sq=1, sk=1500, h=8, hk=2, two_sided=False, causal=True, kv_len=[1500, 1, 600], start=[1499, 300, 599]),
+    dict(b=1, sq=2, sk=3000, h=4, hk=1, two_sided=True)])
+@pytest.mark.parametrize('maps,d,low,near', LEVELS)
+def test_rows_whose_keys_all_carry_one_extreme_bias(maps, d, low, near, shape, dtype):
+    s = dict(shape)
+    x = make(s.pop('b'), s.pop('sq'), s.pop('sk'), h := s.pop('h'), s.pop('hk'), d, dtype, maps, seed=41)
+    level_check(x, maps, torch.full((8, h), max(low, torch.finfo(dtype).min), dtype=dtype), torch.zeros(8, h), 60, **s)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('shape', [
+    dict(b=1, sq=140, sk=200, h=4, hk=2, start=100),                      # the first 60 rows see distance 0, the last 40 start 40 behind the keys
+    dict(b=64, sq=40, sk=64, h=4, hk=4, start=30),
+    dict(b=40, sq=131, sk=300, h=4, hk=2, start=0, kv_len=[300, 40, 0, 90] * 10),     # padded: rows far behind their sequence's end
+    dict(b=3, sq=1, sk=1500, h=8, hk=2, kv_len=[1500, 700, 600], start=[1499, 900, 640]),
+    dict(b=2, sq=3, sk=3000, h=4, hk=1, kv_len=[2900, 3000], start=[2905, 2997])])
+@pytest.mark.parametrize('two_sided', [False, True])
+@pytest.mark.parametrize('maps,d,low,near', LEVELS)
+def test_rows_that_see_an_extreme_bias_beside_others_or_alone(maps, d, low, near, two_sided, shape, dtype):
+    """One-sided and causal, or both sides: keys at distance 8 and more (8 buckets a side, up to 60) carry the extreme."""
+    s = dict(shape)
+    x = make(s.pop('b'), s.pop('sq'), s.pop('sk'), h := s.pop('h'), s.pop('hk'), d, dtype, maps, seed=42)
+    table = torch.randn(16 if two_sided else 8, h, generator=torch.Generator().manual_seed(3))
+    equal = table.clone()
+    for side in range(0, table.shape[0], 8):                       # in every head but the first
+        table[side + 5:side + 8, 1:], equal[side + 5:side + 8, 1:] = low, near
+    level_check(x, maps, table, equal, 60, two_sided, causal=not two_sided, **s)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps', [1, 2])
+@pytest.mark.parametrize('high,low', [(-1e9, -2e9), (-3.0e38, torch.finfo(FP).min), (-1000.0, -2000.0), (3.0e38, -3.0e38)])
+def test_the_larger_of_two_extremes_wins(high, low, maps, dtype):
+    """Distances from 8 on at one level, from 31 on at a lower one; most rows see nothing nearer."""
+    for b, sq, sk in ((1, 100, 90), (70, 40, 90)):
+        x = make(b, sq, sk, 4, 2, 64, dtype, maps, seed=43)
+        table, equal = torch.zeros(8, 4), torch.zeros(8, 4)
+        table[5:7], equal[5:7] = high, 200.0 if high > 0 else -200.0
+        table[7], equal[7] = low, -400.0
+        level_check(x, maps, table, equal, 60, False, True, start=sk + 4)
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+def test_a_nan_in_the_table_reaches_the_rows_that_see_it(dtype):
+    x = make(1, 60, 80, 2, 2, 64, dtype, 1, 8, seed=44)
+    x['bias'] = torch.zeros(8, 2, device='cuda')
+    x['bias'][7, 1] = float('nan')                                        # distances of 31 and more
+    for start in (20, 200):
+        out = call(x, 1, max_distance=60, bidirectional=False, causal=True, query_start=start)
+        sees = start + torch.arange(60) >= 200 if start == 200 else start + torch.arange(60) >= T.bucket_borders(8, 60)[-1]
+        assert torch.isnan(out[0, :, 1]).all(-1).cpu().equal(sees) and not torch.isnan(out[0, :, 0]).any()
