@@ -158,12 +158,17 @@ def load() -> C.CDLL:
             f'{LIB_PATH} is missing: build it with `python -m eo_vae_amd.build` '
             '(eo_vae_amd has no CPU/PyTorch fallback for its kernels)')
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)  # AttributeError if the .so lacks a declared symbol
-        fn.restype, fn.argtypes = res, args
     if lib.eovae_abi_version() != ABI_VERSION:
         raise EovaeError(f'{LIB_PATH} has C-ABI version {lib.eovae_abi_version()}, this package binds '
                          f'version {ABI_VERSION}: rebuild with `python -m eo_vae_amd.build`')
+    # entries are added without a new version (only a changed signature bumps it): an older library may lack some
+    missing = [name for name in SIGNATURES if not hasattr(lib, name)]
+    if missing:
+        raise EovaeError(f'{LIB_PATH} lacks {", ".join(missing)}: it is older than this package; rebuild with '
+                         '`python -m eo_vae_amd.build`')
+    for name, (res, args) in SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
     _lib = lib
     return lib
 

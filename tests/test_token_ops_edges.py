@@ -11,6 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from eo_vae_amd import build as B
+from eo_vae_amd import lib as L
 from eo_vae_amd import token_ops as T
 
 
@@ -110,3 +111,11 @@ def test_no_keys_give_zeros_whatever_the_inputs_hold(maps, dtype, monkeypatch):
     assert out.shape == (2, 0, 2, 64)
     for t, g in zip((keys, bias), torch.autograd.grad(out, (keys, bias), torch.zeros_like(out))):
         assert torch.equal(g, torch.zeros_like(t))
+
+
+def test_a_library_that_lacks_an_entry_is_refused_by_name(monkeypatch):
+    monkeypatch.setattr(L, '_lib', None)
+    monkeypatch.setitem(L.SIGNATURES, 'eovae_of_a_later_day', (C.c_int, []))
+    with pytest.raises(L.EovaeError, match='lacks eovae_of_a_later_day.*rebuild'):
+        L.load()
+    assert L._lib is None
