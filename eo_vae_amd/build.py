@@ -25,12 +25,17 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, '*.hip')) + glob.glob(os.path.join(CSRC, '*.cpp')))
 
 
+def shared():
+    """What every object depends on beside its source: the kernels' headers, the ABI's header and this file (its flags)."""
+    return glob.glob(os.path.join(CSRC, '*.h')) + glob.glob(os.path.join(os.path.dirname(HERE), 'include', '*.h')) + [os.path.abspath(__file__)]
+
+
+def stale(target, deps) -> bool:
+    return not os.path.exists(target) or any(os.path.getmtime(d) >= os.path.getmtime(target) for d in deps)
+
+
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
-        return True
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(CSRC, '*.h'))
-    return any(os.path.getmtime(s) > t for s in deps)
+    return stale(LIB, sources() + shared())
 
 
 def build(force: bool = False, verbose: bool = True) -> str:
@@ -45,9 +50,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     for src in sources():
         obj = os.path.join(HERE, 'build', os.path.basename(src) + '.o')
         objs.append(obj)
-        if (not force and os.path.exists(obj) and os.path.getmtime(obj) > os.path.getmtime(src)
-                and all(os.path.getmtime(obj) > os.path.getmtime(h)
-                        for h in glob.glob(os.path.join(CSRC, '*.h')))):
+        if not force and not stale(obj, [src] + shared()):
             continue
         cmd = [hipcc, f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-c', src, '-o', obj]
         if src.endswith('.hip'):

@@ -119,3 +119,32 @@ def test_a_library_that_lacks_an_entry_is_refused_by_name(monkeypatch):
     with pytest.raises(L.EovaeError, match='lacks eovae_of_a_later_day.*rebuild'):
         L.load()
     assert L._lib is None
+
+
+@pytest.mark.parametrize('newer,rebuilt', [
+    (None, 0), ('pkg/csrc/a.hip', 1), ('pkg/csrc/common.h', 2), ('include/abi.h', 2), ('pkg/build.py', 2)])
+def test_what_makes_a_built_library_stale(newer, rebuilt, tmp_path, monkeypatch):
+    for n in ('pkg/csrc/a.hip', 'pkg/csrc/b.hip', 'pkg/csrc/common.h', 'include/abi.h', 'pkg/build.py', 'pkg/build/a.hip.o', 'pkg/build/b.hip.o',
+              'pkg/lib.so'):
+        f = tmp_path / n
+        f.parent.mkdir(parents=True, exist_ok=True)
+        f.write_text('')
+        os.utime(f, (1000, 1000 + (f.suffix in ('.o', '.so')) + 2 * (n == newer)))
+    for name, path in (('HERE', 'pkg'), ('CSRC', 'pkg/csrc'), ('LIB', 'pkg/lib.so'), ('__file__', 'pkg/build.py')):
+        monkeypatch.setattr(B, name, str(tmp_path / path))
+    ran = []
+
+    class Compiler:
+        returncode = 0
+
+        def __init__(self, cmd, **kw):
+            ran.append(cmd)
+
+        def communicate(self):
+            return b'', None
+    monkeypatch.setattr(B.subprocess, 'Popen', Compiler)
+    monkeypatch.setattr(B.subprocess, 'run', lambda cmd, **kw: None)
+    monkeypatch.setattr(B.shutil, 'which', lambda n: str(tmp_path / 'pkg/lib.so'))          # any file that is there
+    assert B.needs_build() == (newer is not None)
+    B.build(verbose=False)
+    assert len(ran) == rebuilt
