@@ -609,6 +609,9 @@ __global__ __launch_bounds__(256, D == 32 && !SPLIT ? 3 : sizeof(T) == 2 && D * 
   for (int g = 0; g < G && p.bk.n; ++g) wide = wide || uniform(p.wide[hk * G + g]);
   if (wide) walk(std::true_type{}, tid, lane);
   else walk(std::false_type{}, tid, lane);
+  if (!live)                                                       // keys that no query sees take no gradient, not even of a NaN in dO or Q
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) dk[j] = dv[j] = zero16();
   if constexpr (SPLIT) {
     const long long ld = (long long)p.Hkv * D;
     meet_sum<T, D>((float*)lds, dk, p.scale, (T*)p.dk + ((size_t)b * p.Sk * p.Hkv + hk) * D, ld, klo, p.Sk, wave, lane);

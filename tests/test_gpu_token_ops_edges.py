@@ -156,3 +156,22 @@ def test_a_nan_in_the_table_reaches_the_rows_that_see_it(dtype):
         out = call(x, 1, max_distance=60, bidirectional=False, causal=True, query_start=start)
         sees = start + torch.arange(60) >= 200 if start == 200 else start + torch.arange(60) >= T.bucket_borders(8, 60)[-1]
         assert torch.isnan(out[0, :, 1]).all(-1).cpu().equal(sees) and not torch.isnan(out[0, :, 0]).any()
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps,d', [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)])
+@pytest.mark.parametrize('b,sq,sk,h,hk,causal,start,lens', [
+    (1, 40, 90, 2, 2, False, 0, [70]), (1, 40, 90, 2, 1, True, 20, None), (1, 333, 210, 6, 1, False, 0, [150]),
+    (64, 37, 75, 4, 4, False, 0, [75, 0, 40, 64] * 16)])
+def test_keys_that_no_query_sees_take_no_gradient_of_a_nan(b, sq, sk, h, hk, causal, start, lens, maps, d, dtype):
+    x = make(b, sq, sk, h, hk, d, dtype, maps, 8, seed=45)
+    x['do'][:, sq // 2, 0, 3] = float('nan')
+    x['q'][:, sq - 1] = float('inf')
+    leaves = [x[n].requires_grad_(True) for n in ('k', 'v')]
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device='cuda')
+    out = call(x, maps, max_distance=20, causal=causal, bidirectional=not causal, query_start=start, kv_len=n)
+    for g in torch.autograd.grad(out, leaves, x['do']):
+        for i in range(b):
+            last = start + sq if causal else lens[i]
+            assert torch.equal(g[i, last:], torch.zeros_like(g[i, last:]))
+            assert last == 0 or torch.isnan(g[i, :last]).any()
