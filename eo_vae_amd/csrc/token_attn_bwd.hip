@@ -258,6 +258,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   };
   if (wide) walk(std::true_type{});        // a loop of its own: in one loop with the ordinary tiles it cost those 3 to 5 %
   else walk(std::false_type{});
+  if (min(kend - 1, p.causal ? qpos : 0x7fffffff) < 0)               // a query that sees no key takes no gradient, whatever keys and values hold
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[j] = zero16();
   if constexpr (SPLIT) {
     // the waves' sums over their keys: statistics into every wave, the output tile through the same LDS
     float* st = (float*)lds;

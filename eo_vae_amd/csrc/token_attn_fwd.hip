@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
   l = column_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) acc[j] *= inv;
+  for (int j = 0; j < D / 32; ++j) acc[j] = l == 0.f ? zero16() : acc[j] * inv;      // a row that sees no key: 0 whatever the values hold
   if (p.lse && live && half == 0)
     p.lse[(((size_t)b * p.H + h) * MAPS + map) * p.Sq + qrow] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
   const size_t orow = (((size_t)b * p.Sq + qrow) * p.H + h) * D;
@@ -463,6 +463,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
     __syncthreads();
     const float lt = column_sum(l[a]);
     const int col = lane & 31;
+    if (lt == 0.f)                                             // no key of this wave's: 0 whatever the values hold
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[a][i] = zero16();
     if (half == 0) {
       stat[(wave * 32 + col) * 2] = m[a];
       stat[(wave * 32 + col) * 2 + 1] = lt;

@@ -175,3 +175,17 @@ def test_keys_that_no_query_sees_take_no_gradient_of_a_nan(b, sq, sk, h, hk, cau
             last = start + sq if causal else lens[i]
             assert torch.equal(g[i, last:], torch.zeros_like(g[i, last:]))
             assert last == 0 or torch.isnan(g[i, :last]).any()
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps,d', [(1, 32), (1, 64), (1, 128), (2, 64), (2, 128)])
+@pytest.mark.parametrize('b,h,sq,sk', [(1, 2, 30, 40), (64, 4, 40, 50), (2, 4, 6, 2000)])
+def test_queries_that_see_no_key_stay_zero_beside_keys_that_hold_nan(b, h, sq, sk, maps, d, dtype):
+    """Causal, the first query five positions before the first key: five rows see nothing, the sixth sees a NaN."""
+    x = make(b, sq, sk, h, h, d, dtype, maps, 8, seed=46)
+    x['k'][:, 0], x['v'][:, 0] = float('nan'), float('inf')
+    q = x['q'].requires_grad_(True)
+    out = call(x, maps, max_distance=20, causal=True, bidirectional=False, query_start=-5)
+    (dq,) = torch.autograd.grad(out, [q], x['do'])
+    for t in (out, dq):
+        assert torch.equal(t[:, :5], torch.zeros_like(t[:, :5])) and torch.isnan(t[:, 5:]).any(-1).all()
