@@ -204,8 +204,8 @@ def _attention(what, maps, q, k, v, lam, bias_table, max_distance, bidirectional
     widths = (32, 64, 128) if maps == 1 else (64, 128)
     if not (dim in widths):
         raise ValueError(f'{what}: head width {dim}, wants one of {widths}')
-    if not (max(sq, sk) <= 1 << 28):
-        raise ValueError(f'{what}: {sq} queries, {sk} keys (at most 2^28)')
+    if not (max(sq, sk) <= 1 << 28 and b <= 1 << 20 and h <= 1 << 16):
+        raise ValueError(f'{what}: {sq} queries, {sk} keys (at most 2^28), batch {b} (2^20), {h} heads (2^16)')
     two_sided, borders = False, None
     if bias_table is not None:
         if not (bias_table.dim() == 2 and bias_table.shape[1] == h):
@@ -376,9 +376,9 @@ def gated_norm_residual(h, x, post_weight, gate=None, pre_weight=None, *, post_b
             raise ValueError(f'{what}: gate is {gate.dtype}, the weights {post_weight.dtype}')
         if not (gate.dim() >= 1 and gate.shape[-1] == c and (gate.dim() == 1 or gate.dim() == h.dim()) and lead[:k] == tuple(h.shape[:k])):
             raise ValueError(f'{what}: gate {tuple(gate.shape)} for h {tuple(h.shape)}: [channels], or the shape of h with ones behind its leading axes')
-    if not 0 < float(eps) < math.inf:
+    if not 0 < C.c_float(eps).value < math.inf:                     # as the kernels take it
         raise ValueError(f'{what}: eps {eps}')
-    if not math.isfinite(residual_scale):
+    if not math.isfinite(C.c_float(residual_scale).value):
         raise ValueError(f'{what}: residual_scale {residual_scale}')
     _check_gpu(what, h, x, post_weight, post_bias, pre_weight, pre_bias, gate)
     if h.numel() == 0:

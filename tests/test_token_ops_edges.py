@@ -148,3 +148,14 @@ def test_what_makes_a_built_library_stale(newer, rebuilt, tmp_path, monkeypatch)
     assert B.needs_build() == (newer is not None)
     B.build(verbose=False)
     assert len(ran) == rebuilt
+
+
+def test_arguments_that_the_kernels_cannot_take_are_value_errors():
+    z = torch.zeros
+    with pytest.raises(ValueError, match='batch'):
+        T.rel_pos_attention(*[z(1, 1, 1, 32).expand((1 << 20) + 1, 1, 1, 32)] * 3)
+    with pytest.raises(ValueError, match='heads'):
+        T.rel_pos_attention(*[z(1, 1, 1, 32).expand(1, 1, (1 << 16) + 1, 32)] * 3)
+    for kw, text in ((dict(eps=1e-60), 'eps'), (dict(eps=1e60), 'eps'), (dict(residual_scale=-1e60), 'residual_scale')):
+        with pytest.raises(ValueError, match=text):
+            T.gated_norm_residual(z(3, 16), z(3, 16), z(16), **kw)
