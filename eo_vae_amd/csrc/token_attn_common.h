@@ -410,6 +410,8 @@ static inline int make_params(const eovae_token_attention* d, Params& p, const c
   for (const void* x : ptrs) EOVAE_CHECK_ARG((size_t)x % 16 == 0, "%s: a tensor is not 16-byte aligned", who);
   EOVAE_CHECK_ARG(d->q && d->k && d->v && d->out, "%s: null q, k, v or out", who);
   EOVAE_CHECK_ARG(d->maps == 1 || d->lam, "%s: two maps need lambda", who);
+  EOVAE_CHECK_ARG(!d->bias || d->bias_dtype == EOVAE_F32 || d->bias_dtype == EOVAE_BF16, "%s: bias dtype %d (0 fp32, 1 bf16)", who, d->bias_dtype);
+  EOVAE_CHECK_ARG(!d->lam || d->lam_dtype == EOVAE_F32 || d->lam_dtype == EOVAE_BF16, "%s: lambda dtype %d (0 fp32, 1 bf16)", who, d->lam_dtype);
   EOVAE_CHECK_ARG(isfinite(d->scale), "%s: scale is not finite", who);
   if (backward) {
     EOVAE_CHECK_ARG(d->lse && d->d_out && d->dq && d->dk && d->dv, "%s: null lse, d_out, dq, dk or dv", who);

@@ -159,3 +159,11 @@ def test_arguments_that_the_kernels_cannot_take_are_value_errors():
     for kw, text in ((dict(eps=1e-60), 'eps'), (dict(eps=1e60), 'eps'), (dict(residual_scale=-1e60), 'residual_scale')):
         with pytest.raises(ValueError, match=text):
             T.gated_norm_residual(z(3, 16), z(3, 16), z(16), **kw)
+
+
+@pytest.mark.parametrize('kw,text', [(dict(bias=1 << 20, bias_dtype=2), b'bias dtype'), (dict(maps=2, lam=1 << 20, lam_dtype=-1), b'lambda dtype')])
+def test_the_library_refuses_types_of_parameters(kw, text):
+    from test_token_ops_host import attention_descriptor
+    d = attention_descriptor(**kw)
+    for call in (L.load().eovae_token_attention_fwd, L.load().eovae_token_attention_bwd):
+        assert call(C.byref(d), None) == -1 and text in L.load().eovae_last_error()
