@@ -221,6 +221,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
 }
 
 // ---- step form ----
+// Two maps, bf16: the value products are of A = P_0 - mix P_1 and of P_1, with mix an estimate of lambda l_0 / l_1 (each
+// row's own, in the units of its references).  U = sum A v then already is the difference that leaves, its weights rounded once as
+// one map's are, and what the rounding of P_1 puts into W = sum P_1 v counts only as far as the estimate is off:
+//   sum P_0 v = U + mix W      out = (U + mix W) / l_0 - lambda W / l_1
+// (With the maps apart their roundings add up: 4 caches of 8192 .. 32768 keys 2.57e-3 off, now 2.33e-3, which is one map's error
+// too; the final rounding alone is 1.66e-3.  80 us either way.)  It begins with a wave's second tile, which has an estimate: on
+// a walk of one tile the largest weights, which are 1 and not rounded at all, count for more.  mix is set anew when the references
+// move and at tiles 1, 2, 4, 8, ...; a0, a1: the maps' factors then.
+template <typename T, int MAPS> constexpr bool mixes() { return MAPS == 2 && sizeof(T) == 2; }
+template <int J>
+__device__ __forceinline__ void move_mix(f32x16 (&u)[J], f32x16 (&w)[J], float& mix, float a0, float a1, float l0, float l1, float lam) {
+  l0 = column_sum(l0);
+  l1 = column_sum(l1);
+  const float next = l0 > 0.f && l1 > 0.f ? fminf(fmaxf(lam * l0 / l1, -65536.f), 65536.f) : 0.f;       // any finite value is right
+  const float k = a0 * mix - a1 * next;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    u[j] = a0 * u[j] + k * w[j];
+    w[j] *= a1;
+  }
+  mix = next;
+}
 // part (fp32): per (b, key head, row block, split, map): [32 rows][D] unnormalised sums, then per row (maximum, sum)
 template <int D, int MAPS> constexpr int part_floats() { return MAPS * 32 * (D + 2); }
 
@@ -368,6 +390,8 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
     for (int i = 0; i < D / 32; ++i) acc[a][i] = zero16();
   }
   const float c = positive_scale(p.scale, qf);
+  float lam = 0.f, mix = 0.f;
+  if constexpr (MAPS == 2) lam = ldf(p.lam, h, p.lam_f32);
   for (int flip = 0; k0 < k_hi; k0 += 32 * WAVES, flip ^= 1) {
     char *wk = mine + flip * 2 * T32, *wv = wk + T32;
     wait_reads();
@@ -417,14 +441,18 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
       al[a] = fmaf(column_max(top), cc, off);
       up = up || al[a] > m[a] + SLACK;
     }
-    if (__any(up)) {
+    const bool moved = __any(up);
 #pragma unroll
-      for (int a = 0; a < MAPS; ++a) {
-        const float mn = fmaxf(m[a], al[a]), f = exp2_(m[a] - (mn == -INFINITY ? 0.f : mn));
+    for (int a = 0; a < MAPS; ++a) {
+      const float mn = moved ? fmaxf(m[a], al[a]) : m[a];
+      al[a] = 1.f;
+      if (moved) {
+        al[a] = exp2_(m[a] - (mn == -INFINITY ? 0.f : mn));
         m[a] = mn;
-        l[a] *= f;
+        l[a] *= al[a];
+        if constexpr (!mixes<T, MAPS>())
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[a][i] *= f;
+          for (int i = 0; i < D / 32; ++i) acc[a][i] *= al[a];
       }
     }
 #pragma unroll
@@ -437,6 +465,12 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
         sum += s[a][r];
       }
       l[a] += sum;
+    }
+    if constexpr (mixes<T, MAPS>()) {
+      const int n = (k0 - k_lo) / (32 * WAVES);
+      if (moved || (n > 0 && (n & (n - 1)) == 0)) move_mix(acc[0], acc[1], mix, al[0], al[1], l[0], l[1], n > 0 ? lam : 0.f);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = fmaf(-mix, s[1][r], s[0][r]);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -451,6 +485,9 @@ __global__ __launch_bounds__((64 * step_waves<T, D>())) void attn_step_kernel(co
       }
     }
   }
+  if constexpr (mixes<T, MAPS>())
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[0][i] += mix * acc[1][i];
   // join the waves: [wave][32 rows][D + 4] sums and [wave][32][2] statistics, one map at a time
   constexpr int MROW = D + 4;
   float* meet = (float*)lds;

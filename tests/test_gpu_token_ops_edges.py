@@ -189,3 +189,20 @@ def test_queries_that_see_no_key_stay_zero_beside_keys_that_hold_nan(b, h, sq, s
     (dq,) = torch.autograd.grad(out, [q], x['do'])
     for t in (out, dq):
         assert torch.equal(t[:, :5], torch.zeros_like(t[:, :5])) and torch.isnan(t[:, 5:]).any(-1).all()
+
+
+def rms_off(got, want):
+    return float((got.double().cpu() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize('sk', [4096, 16000])
+def test_two_maps_over_a_long_cache_round_like_one(sk):
+    """bf16, lambda 0.8: a rounding to 8 bits is off by 1.66e-3 rms of values whose mantissas are spread evenly over a binade's logarithm.
+    Weights and output rounded once: sqrt(2) times that, 2.35e-3.  Weights of two maps rounded apart, the second's counting 0.8 and
+    both positive where the difference is not: 2.53e-3 and more.  A wave's first tile of at least four is still apart, so at most
+    sqrt((3 * 2.35^2 + 2.65^2) / 4) = 2.43e-3."""
+    x = make(4, 1, sk, 16, 8, 128, BF, 2, seed=47)
+    x['lam'] = torch.full((16,), 0.8, device='cuda')
+    out = call(x, 2)
+    val, _ = reference(x['q'], x['k'], x['v'], x['do'], 2, 64 ** -0.5, None, x['lam'])
+    assert rms_off(out, val['out']) < 2.43e-3
