@@ -107,6 +107,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   }
   d1 = column_sum(d1);
   d2 = column_sum(d2);
+  const bool sums = p.part || p.lam_part;                          // sum P dA is formed anyway
   float lse[MAPS], delta[MAPS];
   delta[0] = d1;
   if constexpr (MAPS == 2) delta[1] = -lam * d2;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   for (int a = 0; a < MAPS; ++a) {
     const size_t at = (((size_t)b * p.H + h) * MAPS + a) * p.Sq + qrow;
     lse[a] = live ? p.lse[at] : INFINITY;
-    if (live && half == 0 && (!SPLIT || wave == 0)) p.delta[at] = delta[a];
+    if (!sums && live && half == 0 && (!SPLIT || wave == 0)) p.delta[at] = delta[a];
   }
   float base = 0.f;
   bool wide = false;
@@ -138,7 +139,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   float x[MAPS], m[MAPS], xl[MAPS], xr[MAPS], ml[MAPS], mr[MAPS], far_l = 0.f, far_r = 0.f;
 #pragma unroll
   for (int a = 0; a < MAPS; ++a) x[a] = m[a] = xl[a] = xr[a] = ml[a] = mr[a] = 0.f;
-  const bool sums = p.part || p.lam_part;
   // 32 NT keys from position key0 on, their fragments from ka and va
   const auto work = [&](const auto& ka, const auto& va, int key0, auto wide_rows) __attribute__((always_inline)) {
     constexpr bool WIDE_HEAD = decltype(wide_rows)::value;
@@ -281,6 +281,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     m[a] = column_sum(m[a]);
     x[a] = m[a] > 0.f ? x[a] / m[a] : 0.f;
     const float w = a == 0 ? 1.f : -lam;
+    if (sums && live && half == 0 && (!SPLIT || wave == 0)) p.delta[(((size_t)b * p.H + h) * MAPS + a) * p.Sq + qrow] = w * x[a];
     far_l += w * (xl[a] - x[a] * ml[a]);        // both halves: the sum over the wave adds their keys
     far_r += w * (xr[a] - x[a] * mr[a]);
   }
@@ -612,7 +613,9 @@ __global__ __launch_bounds__(256, D == 32 && !SPLIT ? 3 : sizeof(T) == 2 && D * 
   for (int g = 0; g < G && p.bk.n; ++g) wide = wide || uniform(p.wide[hk * G + g]);
   if (wide) walk(std::true_type{}, tid, lane);
   else walk(std::false_type{}, tid, lane);
-  if (!live)                                                       // keys that no query sees take no gradient, not even of a NaN in dO or Q
+  int end = limit;
+  asm volatile("" : "+s"(end));                                     // compared anew, for the same reason as above
+  if (krow >= end)                                                  // keys that no query sees take no gradient, not even of a NaN in dO or Q
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) dk[j] = dv[j] = zero16();
   if constexpr (SPLIT) {
