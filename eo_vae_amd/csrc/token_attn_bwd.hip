@@ -120,9 +120,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   float base = 0.f;
   bool wide = false;
   if (p.bk.n) {
+    fill_bias(p, tab, h, tid, 256, false);                             // does not wait for what is hardly ever so
     wide = wide_head(p, h, lane);
-    fill_bias(p, tab, h, tid, 256, wide);
-    if (wide) base = row_base(p, h, qpos, kend);
+    if (wide) {
+      fill_bias(p, tab, h, tid, 256, true);
+      base = row_base(p, h, qpos, kend);
+    }
     if (tid == 0 && b == 0 && tile == 0) p.wide[h] = wide;
     if (wide && live && half == 0 && (!SPLIT || wave == 0)) p.base[((size_t)b * p.H + h) * p.Sq + qrow] = base;
     if (p.part) {

@@ -151,9 +151,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (D <= 64 ? 4 : MAPS == 2 ? 3 
   float base = 0.f;
   bool wide = false;
   if (p.bk.n) {
+    fill_bias(p, tab, h, tid, 256, false);                             // does not wait for what is hardly ever so
     wide = wide_head(p, h, lane);
-    fill_bias(p, tab, h, tid, 256, wide);
-    if (wide) base = row_base(p, h, qpos, kend);
+    if (wide) {
+      fill_bias(p, tab, h, tid, 256, true);
+      base = row_base(p, h, qpos, kend);
+    }
   }
   f32x16 acc[D / 32];
 #pragma unroll
