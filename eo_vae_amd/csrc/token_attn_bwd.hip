@@ -5,8 +5,9 @@
 //   dQ_m = scale dS_m K_m    dK_m = scale dS_m^T Q_m    dV = (sum_m w_m P_m)^T dO
 //   dbias[bucket] = sum of dS_0 (+ dS_1) over its pairs       dlambda = - sum dO o O_1
 //
-// delta comes from stored outputs, rounded to the tensors' type: good for dQ and dK, whose sums it enters with the mean of K
-// (of Q) only, but not for the two sums that it could drown.  The last buckets hold nearly all of a long row's probability, and
+// delta comes from stored outputs, rounded to the tensors' type: good for dQ, whose sum it enters with the mean of K only (the row's
+// own sum P dA is known when the pass is over: dK/dV takes that one where it is formed), but not for the two sums that it could
+// drown.  The last buckets hold nearly all of a long row's probability, and
 // there sum dS = w (sum P dA - (mean of dA over the WHOLE row) (sum P)) is a difference of large values; lambda's gradient is
 // that mean.  Both are formed in fp32 from P and dA themselves, row by row; the mean is divided by the row's own sum of P, so that
 // a common error of P's scale (lse's rounding) cancels.
@@ -16,8 +17,8 @@
 // walks the queries of every head that shares its key head, so shared heads' gradients are summed in a fixed order.  The
 // scores are formed in both passes (7 products instead of 5): the price of bit-reproducible gradients without a
 // [queries][keys] buffer.  Bound by vector instructions (exp2, the gradients' two operations per score, conversions) beside the
-// matrix pipes.  bf16, measured: 16 x 8 heads x 1024 x 64 dQ 78 us (664 TFLOP/s of its three products), 115 with the bias gradient,
-// dK/dV 97 (711 of four); 4 x 8 x 2048 x 128 dQ 121 us (850), dK/dV 174 (790); two maps of the same size 161 and 289.
+// matrix pipes.  bf16, measured: 16 x 8 heads x 1024 x 64 dQ 82 us (630 TFLOP/s of its three products), 110 .. 119 with the bias
+// gradient, dK/dV 105 .. 112 (620 of four); 4 x 8 x 2048 x 128 dQ 127 us (810), dK/dV 201 (680); two maps of the same size 162 and 301.
 // No kernel here may spill: hipcc 7.2 has brought a value spilled half to registers, half to scratch back with a register missing.
 #include <math.h>
 #include <type_traits>

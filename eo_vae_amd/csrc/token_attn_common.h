@@ -9,6 +9,17 @@
 // + r % 4, r < 16: eight consecutive registers are a B operand of the next product whose k run {4h..4h+3, 8+4h..8+4h+3}
 // (h = l / 32), so probabilities and score gradients go from one product into the next without leaving their lane, as long
 // as the A operand is read in that order (frag_t below).
+//
+// What is rounded to fewer bits than fp32 where the tensors are bf16 (fp32 tensors: nothing).  The matrix instructions that keep up
+// take 16-bit operands, so what is formed in between enters the next product as bf16, each value rounded once:
+//   unnormalised probabilities, for O (each map's own in the row form; the step form subtracts the maps first);
+//   w_0 P_0 + w_1 P_1, subtracted in fp32, for dV;        score gradients, for dQ and dK;
+//   O and O_1 as they are stored, for the delta of dQ and the near buckets' bias gradient (of dK too where no row sums are formed).
+// Scores, statistics, sums, the difference of two maps and everything the table's far buckets and lambda get stay in fp32.
+// Measured against 64 bits (rms, relative; rounding only the result is 1.66e-3): one map's output, dV and dK 2.35e-3, dQ 2.4e-3 (2.7e-3
+// on rows of some hundred keys); two maps' output 2.33e-3 in the step form, 2.4e-3 .. 2.55e-3 in the row form.  What exact
+// weights would take was measured for two maps: a second product with what the rounding left takes them to 1.9e-3, and 16 x 8 x
+// 1024 x 64 from 53 to 69 us; both maps in one wave, subtracted first, to 2.34e-3, and 16 x 1000 x 8 x 128 from 108 to 133.
 #pragma once
 #include <math.h>
 #include "eovae_common.h"
@@ -18,9 +29,7 @@ namespace tok {
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int MAX_BUCKETS = 128;       // per side: at most 64 borders behind the exact half

@@ -6,11 +6,11 @@
 // map 1 of the same rows (same K / V tiles, half of K's columns each) and meet once at the end.  One wave reads 32 KiB of LDS
 // for 1024 cycles of matrix instructions at 128 columns, which is what the four waves' share of the LDS gives, and 32 exp2 at a
 // quarter of the vector rate beside them; two waves per SIMD overlap the three.  Measured: 16 heads x 8191 causal x 128
-// columns 295 us (930 TFLOP/s), 16 x 8 x 1024 x 64 55 us without a bias (630), two maps 16 x 8 x 1000 ragged 105 us.
+// columns 301 us (910 TFLOP/s), 16 x 8 x 1024 x 64 57 us without a bias (600), two maps 16 x 8 x 1000 ragged 105 .. 126 us.
 // Step form (few rows per key head, e.g. single tokens against a cache, or a call too small to fill the chip): the rows are the
 // query heads that share one key head times the query tokens, 32 of them to a block, the four waves take different keys, the
 // key axis is also split over blocks where it is long, and then a second kernel joins the partial sums.  Bound by bytes where a
-// cache is long: 32 caches of 1024 .. 4096 keys x 4 key heads x 128, bf16, 37 us (4.6 TB/s; copies reach 4.9) and 4 for the join.
+// cache is long: 32 caches of 1024 .. 4096 keys x 4 key heads x 128, bf16, 42 us (4.0 TB/s; copies reach 4.9) and 4 for the join.
 #include <math.h>
 #include <type_traits>
 #include "token_attn_common.h"
@@ -92,6 +92,7 @@ __device__ __forceinline__ float softmax_tile(const Params& p, f32x16 (&s)[NT], 
 }
 
 // One wave's pass over a staged tile of TILE keys: scores of its 32 queries, softmax update, O^T += V^T P^T.
+// Probabilities enter the value product in the tensors' type (to_frag): bf16 rounds each once.
 // r0: first row of the tile in LDS, key0: its position; qpos: this lane's query position; limit: keys visible at all.
 template <typename T, int D, int MAPS> constexpr int row_tile() { return sizeof(T) == 2 && D == 128 && MAPS == 2 ? 32 : tile_rows<T, D>(); }
 template <typename T, int D, int R, int W, int NT, bool WIDE_HEAD>

@@ -11,7 +11,7 @@
 // Backward:  a = dz w2,  D = dy + rstd_2 (a - mean(a) - t mean(a t)),  dx = alpha D,  c = D g w1,
 //            dh = rstd_1 (c - mean(c) - u mean(c u)),   dw2 = sum dz t,  A = sum D u,  B = sum D  over a gate row's tokens,
 //            dg = w1 A + b1 B,   dw1 = sum over gate rows of g A,   db1 of g B.
-// Measured, bf16: 32768 x 4096 forward 200 us (5.4 TB/s), backward 333 (4.8, six rows of it); 16 x 1024 x 1024 31 and 39 us;
+// Measured, bf16: 32768 x 4096 forward 199 us (5.4 TB/s), backward 352 (4.6, six rows of it); 16 x 1024 x 1024 36 and 39 us;
 // 16 x 2048 5 us.  The next row's loads are in flight while a row is worked on (without: 271 and 899 us at 32768 x 4096).
 // Column sums stay in registers over a block's rows, go through one fp32 partial per block and are folded in a fixed order.
 #include <math.h>
