@@ -614,7 +614,10 @@ __global__ __launch_bounds__(256, D == 32 && !SPLIT ? 3 : sizeof(T) == 2 && D * 
     }
   };
   bool wide = false;                                               // one of the key head's heads is
-  for (int g = 0; g < G && p.bk.n; ++g) wide = wide || uniform(p.wide[hk * G + g]);
+  if (p.bk.n) {
+    for (int g = lane; g < G; g += 64) wide = wide || p.wide[hk * G + g];
+    wide = __any(wide);
+  }
   if (wide) walk(std::true_type{}, tid, lane);
   else walk(std::false_type{}, tid, lane);
   int end = limit;
