@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
   for (int a = 0; a < MAPS; ++a) {
     x[a] = column_sum(x[a]);
     m[a] = column_sum(m[a]);
-    x[a] = m[a] > 0.f ? x[a] / m[a] : 0.f;
+    x[a] = m[a] == 0.f ? 0.f : x[a] / m[a];     // a NaN stays one
     const float w = a == 0 ? 1.f : -lam;
     if (sums && live && half == 0 && (!SPLIT || wave == 0)) p.delta[(((size_t)b * p.H + h) * MAPS + a) * p.Sq + qrow] = w * x[a];
     far_l += w * (xl[a] - x[a] * ml[a]);        // both halves: the sum over the wave adds their keys

@@ -219,3 +219,19 @@ def test_key_gradients_are_rounded_twice_and_no_more(maps, d):
     w = d // maps
     val, _ = reference(x['q'], x['k'], x['v'], x['do'], maps, w ** -0.5, x['bias'], x['lam'])
     assert rms_off(dk, val['dk']) < 2.42e-3
+
+
+@pytest.mark.parametrize('dtype', [FP, BF])
+@pytest.mark.parametrize('maps', [1, 2])
+@pytest.mark.parametrize('b,sq,sk', [(1, 40, 60), (64, 40, 60)])
+def test_a_nan_key_reaches_all_gradients_of_the_rows_that_see_it(b, sq, sk, maps, dtype):
+    """Its softmax has no value, whether or not the call also asks for the parameters' gradients."""
+    x = make(b, sq, sk, 4, 4, 64, dtype, maps, 8, seed=49)
+    x['k'][:, 7] = float('nan')
+    for names in (('q', 'k', 'v'), ('q', 'k', 'v', 'bias') + (('lam',) if maps == 2 else ())):
+        y = {n: None if t is None else t.detach().clone() for n, t in x.items()}
+        leaves = [y[n].requires_grad_(True) for n in names]
+        out = call(y, maps, max_distance=20)
+        assert torch.isnan(out).all()
+        dq, dk = torch.autograd.grad(out, leaves, y['do'])[:2]
+        assert torch.isnan(dq).all() and torch.isnan(dk).all()
